@@ -1,0 +1,365 @@
+// A beam search's step: the K best continuations of the K beams of every request, and the beams'
+// pages moved to where their new parents' are.
+//
+// Selection.  Continuation t of beam j is worth score_j + logit_jt - logsumexp(logit_j); a beam that has
+// ended continues with the end token alone, at its own score.  Taken are the K largest, equal ones by
+// the lowest j V + t.  The values are formed in fp64: they differ between beams by less than fp32 resolves.
+//   pass   one read of the logits: maximum and sum of exponentials of every block of BLK of a row.
+//   pick   one CTA per request.  The K best continuations lie in the K blocks whose best ones are
+//          the best (equal ones by the lowest place): each of those holds one that precedes whatever lies in
+//          another block.  So the blocks' maxima choose K blocks, and only those are read again.
+//
+// Pages.  A request's beams share the pages of what they have in common.  With n tokens stored the next
+// one goes to page n / 64: full pages are taken over from the parent by number; of the children of
+// one parent the first keeps its page of n mod 64 tokens, the others get a free page of the request's pool
+// and a copy.  A page is free when no new row of the request holds it, so nothing is counted from step to step.
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace cb {
+
+constexpr int BEAM_MAX = 32;           // beams of a request
+constexpr int BLK = 1024;              // logits of a block
+constexpr int PICK_THREADS = 256;
+constexpr int PICK_CAP = 1024;         // continuations compared at once
+
+template <typename T>
+__device__ __forceinline__ float beam_logit(const T* p) {
+  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
+  else return *p;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) beam_pass_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk,
+                                                        const float* __restrict__ scores,
+                                                        const uint8_t* __restrict__ done, float2* __restrict__ part) {
+  const int row = blockIdx.y, blk = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (blk >= nblk || done[row] || scores[row] == -INFINITY) return;
+  const T* x = logits + row * ld;
+  const int t0 = blk * BLK, t1 = min(V, t0 + BLK);
+  float m = -INFINITY, s = 0.f;
+  for (int t = t0 + lane; t < t1; t += 32) m = fmaxf(m, beam_logit(x + t));
+  m = warp_max(m);
+  for (int t = t0 + lane; t < t1; t += 32) {
+    const float v = beam_logit(x + t);
+    s += v == -INFINITY ? 0.f : expf(v - m);             // NaN and +inf make the sum NaN
+  }
+  s = warp_sum(s);
+  if (lane == 0) part[static_cast<size_t>(row) * nblk + blk] = make_float2(m, s);
+}
+
+struct Best {              // a continuation or a block: larger value first, then the lower place
+  double v;
+  int64_t at;
+};
+__device__ __forceinline__ bool better(double v, int64_t at, const Best& b) { return v > b.v || (v == b.v && at < b.at); }
+__device__ __forceinline__ Best block_best(Best b, Best* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double v = __shfl_xor_sync(0xffffffffu, b.v, o);
+    const int64_t at = __shfl_xor_sync(0xffffffffu, b.at, o);
+    if (better(v, at, b)) b = Best{v, at};
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = b;
+  __syncthreads();
+  b = red[0];
+  for (int w = 1; w < PICK_THREADS / 32; ++w)
+    if (better(red[w].v, red[w].at, b)) b = red[w];
+  return b;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PICK_THREADS)
+beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int K, const float* __restrict__ scores,
+                 const uint8_t* __restrict__ done, int eos, const float2* __restrict__ part,
+                 float* __restrict__ out_score, int64_t* __restrict__ out_parent, int64_t* __restrict__ out_token,
+                 uint8_t* __restrict__ out_done) {
+  __shared__ Best red[PICK_THREADS / 32];
+  __shared__ double s_lse[BEAM_MAX];
+  __shared__ int64_t s_blk[BEAM_MAX];
+  __shared__ double c_v[PICK_CAP];
+  __shared__ int64_t c_at[PICK_CAP];
+  __shared__ int s_n;
+  const int item = blockIdx.x, row0 = item * K;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const double NEG = -INFINITY;
+  for (int j = warp; j < K; j += PICK_THREADS / 32) {
+    const float2* p = part + static_cast<size_t>(row0 + j) * nblk;
+    double lse = NEG;
+    if (!done[row0 + j] && scores[row0 + j] != -INFINITY) {
+      float m = -INFINITY;
+      for (int i = lane; i < nblk; i += 32) m = fmaxf(m, p[i].x);
+      m = warp_max(m);
+      double s = 0.0;
+      for (int i = lane; i < nblk; i += 32) {
+        const float2 q = p[i];
+        s += q.x == -INFINITY && q.y == 0.f ? 0.0 : static_cast<double>(q.y) * exp(static_cast<double>(q.x) - static_cast<double>(m));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      lse = static_cast<double>(m) + log(s);
+    }
+    if (lane == 0) s_lse[j] = lse;
+  }
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  // the value of a logit of beam j; what is not a number is no continuation
+  auto value = [&](int j, float x) {
+    const double v = static_cast<double>(scores[row0 + j]) + (static_cast<double>(x) - s_lse[j]);
+    return v == v ? v : NEG;
+  };
+  // the K best blocks, one after the other; an ended beam is one block
+  int found = 0;
+  Best last{INFINITY, -1};
+  for (; found < K; ++found) {
+    Best b{NEG, 0x7fffffffffffffffll};
+    for (int i = threadIdx.x; i < K * nblk; i += PICK_THREADS) {
+      const int j = i / nblk, k = i % nblk;
+      double v = NEG;
+      if (done[row0 + j]) {
+        if (k == 0 && eos >= 0) v = scores[row0 + j];
+        if (v != v) v = NEG;
+      } else if (scores[row0 + j] != -INFINITY) {
+        v = value(j, part[static_cast<size_t>(row0 + j) * nblk + k].x);
+      }
+      if (v > NEG && better(v, i, b) && !better(v, i, last) && i != last.at) b = Best{v, i};
+    }
+    b = block_best(b, red);
+    if (!(b.v > NEG)) break;
+    if (threadIdx.x == 0) s_blk[found] = b.at;
+    last = b;
+  }
+  __syncthreads();
+  const double least = found == K ? last.v : NEG;
+  // every continuation of those blocks that is not below the last block's best
+  auto each = [&](auto&& f) {
+    for (int n = 0; n < found; ++n) {
+      const int j = static_cast<int>(s_blk[n] / nblk), k = static_cast<int>(s_blk[n] % nblk);
+      if (done[row0 + j]) {
+        if (threadIdx.x == 0) f(static_cast<double>(scores[row0 + j]), static_cast<int64_t>(j) * V + eos);
+        continue;
+      }
+      const T* x = logits + (row0 + j) * ld;
+      const int t1 = min(V, (k + 1) * BLK);
+      for (int t = k * BLK + threadIdx.x; t < t1; t += PICK_THREADS) f(value(j, beam_logit(x + t)), static_cast<int64_t>(j) * V + t);
+    }
+  };
+  each([&](double v, int64_t at) {
+    if (v >= least && v > NEG) {
+      const int n = atomicAdd(&s_n, 1);
+      if (n < PICK_CAP) {
+        c_v[n] = v;
+        c_at[n] = at;
+      }
+    }
+  });
+  __syncthreads();
+  const int n = s_n;
+  auto put = [&](int place, double v, int64_t at) {
+    const int j = static_cast<int>(at / V), t = static_cast<int>(at % V);
+    out_score[row0 + place] = static_cast<float>(v);
+    out_parent[row0 + place] = j;
+    out_token[row0 + place] = t;
+    out_done[row0 + place] = done[row0 + j] || t == eos;
+  };
+  int filled;
+  if (n <= PICK_CAP) {
+    // a continuation's place is the number of those before it
+    for (int i = threadIdx.x; i < n; i += PICK_THREADS) {
+      int rank = 0;
+      const Best me{c_v[i], c_at[i]};
+      for (int o = 0; o < n; ++o) rank += better(c_v[o], c_at[o], me);
+      if (rank < K) put(rank, me.v, me.at);
+    }
+    filled = min(n, K);
+  } else {
+    // more equal ones than that: one after the other
+    Best prev{INFINITY, -1};
+    for (filled = 0; filled < K; ++filled) {
+      Best b{NEG, 0x7fffffffffffffffll};
+      each([&](double v, int64_t at) {
+        if (v > NEG && better(v, at, b) && !better(v, at, prev) && at != prev.at) b = Best{v, at};
+      });
+      b = block_best(b, red);
+      if (!(b.v > NEG)) break;
+      if (threadIdx.x == 0) put(filled, b.v, b.at);
+      prev = b;
+    }
+  }
+  for (int i = filled + threadIdx.x; i < K; i += PICK_THREADS) {      // places left: dead beams
+    out_score[row0 + i] = -INFINITY;
+    out_parent[row0 + i] = i;
+    out_token[row0 + i] = max(eos, 0);
+    out_done[row0 + i] = 1;
+  }
+}
+
+// ------------------------------------------------------------------------------------ pages
+constexpr int BEAM_PAGE = 64;
+
+// One CTA per request.  used: one bit per page of the cache, in shared memory.
+__global__ void __launch_bounds__(256) beam_pages_kernel(const int* __restrict__ table, int width, int K,
+                                                         const int64_t* __restrict__ parent,
+                                                         const int* __restrict__ length, const int* __restrict__ pool,
+                                                         int pool_n, int num_pages, int* __restrict__ out,
+                                                         int* __restrict__ src, int* __restrict__ dst, int* status) {
+  extern __shared__ uint32_t used[];
+  __shared__ int s_parent[BEAM_MAX], s_keeps[BEAM_MAX], s_free[BEAM_MAX], s_turn[BEAM_MAX];
+  const int item = blockIdx.x, row0 = item * K;
+  const int len = length[item], lp = len / BEAM_PAGE;
+  const bool partial = len % BEAM_PAGE != 0;
+  if (len < 0 || lp >= width) {                       // no place for the next token
+    for (int i = threadIdx.x; i < K * width; i += blockDim.x) out[static_cast<size_t>(row0) * width + i] = table[static_cast<size_t>(row0) * width + i];
+    for (int j = threadIdx.x; j < K; j += blockDim.x) src[row0 + j] = dst[row0 + j] = -1;
+    if (threadIdx.x == 0) record_status(status, ST_BOUNDS, item);
+    return;
+  }
+  for (int i = threadIdx.x; i < (num_pages + 31) / 32; i += blockDim.x) used[i] = 0u;
+  if (threadIdx.x < K) {
+    int64_t p = parent[row0 + threadIdx.x];
+    if (p < 0 || p >= K) {
+      record_status(status, ST_BOUNDS, item);
+      p = threadIdx.x;
+    }
+    s_parent[threadIdx.x] = static_cast<int>(p);
+  }
+  __syncthreads();
+  if (threadIdx.x < K) {
+    bool keeps = partial;
+    for (int j = 0; j < threadIdx.x; ++j) keeps = keeps && s_parent[j] != s_parent[threadIdx.x];
+    s_keeps[threadIdx.x] = keeps;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int j = 0; j < K; ++j) {
+      s_turn[j] = n;
+      n += !s_keeps[j];
+      s_free[j] = -1;
+    }
+  }
+  auto mark = [&](int page) {
+    if (page >= 0 && page < num_pages) atomicOr(&used[page / 32], 1u << (page % 32));
+  };
+  for (int i = threadIdx.x; i < K * width; i += blockDim.x) {
+    const int j = i / width, c = i % width;
+    const size_t at = static_cast<size_t>(row0 + j) * width + c;
+    const int theirs = table[static_cast<size_t>(row0 + s_parent[j]) * width + c];
+    if (c < lp || (c == lp && s_keeps[j])) {
+      out[at] = theirs;
+      mark(theirs);
+    } else if (c > lp) {
+      out[at] = table[at];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {                              // the first K free pages, in the pool's order
+    int n = 0;
+    for (int i0 = 0; i0 < pool_n && n < K; i0 += 32) {
+      const int i = i0 + threadIdx.x;
+      const int page = i < pool_n ? pool[static_cast<size_t>(item) * pool_n + i] : -1;
+      const bool ok = page >= 0 && page < num_pages && !(used[page / 32] >> (page % 32) & 1u);
+      const uint32_t all = __ballot_sync(0xffffffffu, ok);
+      const int place = n + __popc(all & ((1u << threadIdx.x) - 1u));
+      if (ok && place < K) s_free[place] = page;
+      n += __popc(all);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < K) {
+    const int j = threadIdx.x;
+    int s = -1, d = -1;
+    if (!s_keeps[j]) {
+      d = s_free[s_turn[j]];
+      out[static_cast<size_t>(row0 + j) * width + lp] = d;
+      if (partial) s = table[static_cast<size_t>(row0 + s_parent[j]) * width + lp];
+      if (d < 0) record_status(status, ST_BOUNDS, item);       // the pool is too small
+    }
+    const bool copy = s >= 0 && s < num_pages && d >= 0;
+    src[row0 + j] = copy ? s : -1;
+    dst[row0 + j] = copy ? d : -1;
+  }
+}
+
+constexpr int COPY_MAX = 192;          // tensors of one launch
+struct CopyArgs {
+  void* base[COPY_MAX];
+  int bytes[COPY_MAX];                 // of a page, a multiple of 4
+};
+__global__ void __launch_bounds__(256) beam_copy_kernel(const __grid_constant__ CopyArgs a, const int* __restrict__ src,
+                                                        const int* __restrict__ dst) {
+  const int s = src[blockIdx.x], d = dst[blockIdx.x];
+  if (s < 0 || d < 0 || s == d) return;
+  const size_t bytes = a.bytes[blockIdx.y];
+  const char* from = static_cast<const char*>(a.base[blockIdx.y]) + s * bytes;
+  char* to = static_cast<char*>(a.base[blockIdx.y]) + d * bytes;
+  const size_t first = blockIdx.z * static_cast<size_t>(blockDim.x) + threadIdx.x, step = gridDim.z * static_cast<size_t>(blockDim.x);
+  if (((reinterpret_cast<uintptr_t>(a.base[blockIdx.y]) | bytes) & 15) == 0) {
+    for (size_t i = first; i < bytes / 16; i += step) reinterpret_cast<uint4*>(to)[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+  } else {
+    for (size_t i = first; i < bytes / 4; i += step) reinterpret_cast<uint32_t*>(to)[i] = __ldg(reinterpret_cast<const uint32_t*>(from) + i);
+  }
+}
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" int cb_beam_block() { return BLK; }
+
+// part: float2 [B K, ceil(V / cb_beam_block())] scratch
+extern "C" int cb_beam_select(const void* logits, int64_t ld, int f32, int B, int K, int V, const float* scores,
+                              const void* done, int eos, void* part, float* out_score, int64_t* out_parent,
+                              int64_t* out_token, void* out_done, void* stream) {
+  if (B < 1 || K < 1 || K > BEAM_MAX || V < 1 || eos >= V) return -1;
+  const int nblk = (V + BLK - 1) / BLK;
+  if (1ll * B * K > 65535) return -2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid((nblk + 7) / 8, B * K);
+  auto* P = static_cast<float2*>(part);
+  auto* D = static_cast<const uint8_t*>(done);
+  auto* OD = static_cast<uint8_t*>(out_done);
+  auto go = [&](auto* x) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+    beam_pass_kernel<T><<<grid, 256, 0, st>>>(x, ld, V, nblk, scores, D, P);
+    beam_pick_kernel<T><<<B, PICK_THREADS, 0, st>>>(x, ld, V, nblk, K, scores, D, eos, P, out_score, out_parent, out_token, OD);
+  };
+  if (f32) go(static_cast<const float*>(logits));
+  else go(static_cast<const __nv_bfloat16*>(logits));
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+extern "C" int cb_beam_pages(const int* table, int width, int B, int K, const int64_t* parent, const int* length,
+                             const int* pool, int pool_n, int num_pages, int* out, int* src, int* dst, int* status,
+                             void* stream) {
+  if (B < 1 || K < 1 || K > BEAM_MAX || width < 1 || pool_n < 0 || num_pages < 1) return -1;
+  const int bytes = (num_pages + 31) / 32 * 4;
+  if (bytes > 200 * 1024) return -2;
+  if (bytes > 40 * 1024 &&
+      cudaFuncSetAttribute(beam_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return -4;
+  beam_pages_kernel<<<B, 256, bytes, static_cast<cudaStream_t>(stream)>>>(table, width, K, parent, length, pool, pool_n,
+                                                                          num_pages, out, src, dst, status);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// Copies page src[i] to page dst[i] (-1: none) in every tensor; base and bytes are host arrays.
+extern "C" int cb_beam_copy(void* const* base, const int* bytes, int tensors, const int* src, const int* dst, int n,
+                            void* stream) {
+  if (n < 1 || tensors < 1) return -1;
+  for (int t0 = 0; t0 < tensors; t0 += COPY_MAX) {
+    CopyArgs a;
+    const int nt = tensors - t0 < COPY_MAX ? tensors - t0 : COPY_MAX;
+    int most = 0;
+    for (int t = 0; t < nt; ++t) {
+      a.base[t] = base[t0 + t];
+      a.bytes[t] = bytes[t0 + t];
+      if (a.bytes[t] < 4 || a.bytes[t] % 4 != 0) return -2;
+      most = a.bytes[t] > most ? a.bytes[t] : most;
+    }
+    const dim3 grid(n, nt, (most + 16383) / 16384);
+    beam_copy_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a, src, dst);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}

@@ -1,0 +1,295 @@
+"""A paged cache in 8 bits (``csrc/kv8.cu``, ``csrc/kv8_attn.cu``): append, read back, attention.
+
+The cache of one layer is four tensors (:func:`kv8_alloc`).  Pages hold 64 tokens; of a page and
+head the keys are ``[dh / 64][token][64]`` codes, the values ``[dh][token]`` codes, in ``int8`` or
+``float8_e4m3fn``.  A code stands for ``code * scale`` with one scale per page, head and side, the
+smallest power of two (not below 2^-126) under which the block's largest magnitude fits the codes.  A
+page that gets more tokens keeps its scale or takes a larger one, to which its codes are then rounded
+again.  A key or value that is not finite makes its block's scale NaN, so that whatever attends to the
+block is NaN.
+
+``int8`` spends its steps evenly (good for values without outliers), ``float8_e4m3fn`` keeps three
+bits of every number however small.
+
+The entries of a call are sequences: entry ``e`` has page-table row ``e``.  With ``row0 [n + 1]`` it
+owns rows ``row0[e] .. row0[e + 1] - 1`` of the row-wise tensors, at most ``max_rows`` of them
+(possibly none); without, row ``e`` alone.  An entry whose rows, positions or pages are out of range is
+skipped and recorded in the status word (:func:`coeus_b200.ops._lib.check_status`).  Entries of one
+:func:`kv8_write` must not write the same page.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .decode import PAGE
+
+KINDS = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+_QMAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def kv8_alloc(num_pages: int, heads: int, dh: int, kind: str, device
+              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(k_cache, v_cache, k_scale, v_scale)`` of one layer, all zero; ``kind`` is ``"int8"`` or
+    ``"e4m3"``."""
+    if kind not in KINDS:
+        raise ValueError(f"kv8: the codes are int8 or e4m3, not {kind!r}")
+    if dh not in (64, 128):
+        raise ValueError(f"kv8: heads of 64 or 128, not {dh}")
+    k = torch.zeros((num_pages, heads, dh // 64, PAGE, 64), dtype=torch.int8, device=device)
+    v = torch.zeros((num_pages, heads, dh, PAGE), dtype=torch.int8, device=device)
+    s = torch.zeros((2, num_pages, heads), dtype=torch.float32, device=device)
+    return k.view(KINDS[kind]), v.view(KINDS[kind]), s[0], s[1]
+
+
+def _check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, ints, row0, max_rows):
+    """Shapes and types of what every call takes; returns ``(pages, heads, dh)``."""
+    if k_cache.dim() != 5 or k_cache.shape[3:] != (PAGE, 64) or k_cache.dtype not in _QMAX:
+        raise ValueError(f"{what}: keys are [pages, heads, dh / 64, {PAGE}, 64] codes, got "
+                         f"{tuple(k_cache.shape)} {k_cache.dtype}")
+    pages, heads, dh = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2] * 64
+    if dh not in (64, 128):
+        raise ValueError(f"{what}: heads of 64 or 128, not {dh}")
+    if tuple(v_cache.shape) != (pages, heads, dh, PAGE) or v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"{what}: values {tuple(v_cache.shape)} {v_cache.dtype} do not go with "
+                         f"keys {tuple(k_cache.shape)} {k_cache.dtype}")
+    for s in (k_scale, v_scale):
+        if tuple(s.shape) != (pages, heads) or s.dtype != torch.float32:
+            raise ValueError(f"{what}: scales are fp32 [{pages}, {heads}]")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1:
+        raise ValueError(f"{what}: the page table is int32 [entries, pages]")
+    n = page_table.shape[0]
+    if tuple(ints.shape) != (n,) or ints.dtype != torch.int32:
+        raise ValueError(f"{what}: one int32 number per entry, got {tuple(ints.shape)} {ints.dtype}")
+    if row0 is not None and (tuple(row0.shape) != (n + 1,) or row0.dtype != torch.int32):
+        raise ValueError(f"{what}: row0 is int32 [{n + 1}]")
+    if max_rows < 1 or (row0 is None and max_rows != 1):
+        raise ValueError(f"{what}: max_rows is the bound on an entry's rows (1 without row0)")
+    for t in (k_cache, v_cache, k_scale, v_scale, page_table, ints, row0):
+        if t is None:
+            continue
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: cache, tables and lengths have to be contiguous")
+        if t.device != k_cache.device:
+            raise ValueError(f"{what}: tensors on {t.device} and {k_cache.device}")
+    return pages, heads, dh
+
+
+def _rows(what: str, x: torch.Tensor, width: int, like: torch.Tensor) -> torch.Tensor:
+    """A row-wise input as the kernels read it: bf16, unit inner stride, 16-byte rows (a copy where
+    the caller's view is laid out otherwise)."""
+    if x.dim() != 2 or x.shape[1] != width:
+        raise ValueError(f"{what}: rows of {width} numbers, got {tuple(x.shape)}")
+    if x.device != like.device:
+        raise ValueError(f"{what}: tensors on {x.device} and {like.device}")
+    if not x.is_cuda:
+        return x
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: the kernels take bf16 rows, got {x.dtype}")
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16 or x.stride(0) >= 1 << 31:
+        x = x.contiguous()
+    return x
+
+
+def _spans(n: int, row0, rows: int, max_rows: int):
+    """``(entry, first row, rows)`` of the entries that have any, on the host."""
+    if row0 is None:
+        if n > rows:
+            raise ValueError(f"kv8: {n} entries, {rows} rows")
+        return [(e, e, 1) for e in range(n)]
+    at = row0.tolist()
+    out = []
+    for e in range(n):
+        if at[e + 1] > at[e]:
+            if at[e + 1] - at[e] > max_rows or at[e] < 0 or at[e + 1] > rows:
+                raise ValueError(f"kv8: entry {e} has rows {at[e]} .. {at[e + 1] - 1}")
+            out.append((e, at[e], at[e + 1] - at[e]))
+    return out
+
+
+def _exponent(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Smallest ``e >= -126`` with ``amax <= QMAX * 2^e``."""
+    m, x = torch.frexp(amax)
+    e = x - 7 + (m > 127.0 / 128.0).to(x.dtype) if dtype == torch.int8 else \
+        x - 9 + (m > 0.875).to(x.dtype)
+    return torch.where(amax > 0, e, torch.full_like(e, -126)).clamp_min(-126)
+
+
+def _encode(y: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    y = torch.nan_to_num(y, 0.0, 0.0, 0.0)
+    return y.round().to(torch.int8) if dtype == torch.int8 else y.to(dtype)
+
+
+def _block(codes: torch.Tensor, keys: bool) -> torch.Tensor:
+    """Codes of one page ``[heads, ...]`` as fp32 ``[heads, 64, dh]``."""
+    x = codes.float()
+    if keys:
+        return x.transpose(1, 2).reshape(x.shape[0], PAGE, -1)
+    return x.transpose(1, 2)
+
+
+def _values(codes: torch.Tensor, scale: torch.Tensor, page: int, keys: bool) -> torch.Tensor:
+    """Values of one page, fp32 ``[heads, 64, dh]``."""
+    return _block(codes[page], keys) * scale[page][:, None, None]
+
+
+def _cpu_page(table: torch.Tensor, e: int, lp: int, pages: int) -> int:
+    page = int(table[e, lp]) if lp < table.shape[1] else -1
+    if not 0 <= page < pages:
+        raise ValueError(f"kv8: entry {e} has no page {lp}")
+    return page
+
+
+def kv8_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
+              pos0: torch.Tensor, row0: Optional[torch.Tensor] = None, max_rows: int = 1) -> None:
+    """Stores the rows of ``k`` / ``v`` (``[rows, heads * dh]`` views) at positions ``pos0[e]`` and on of
+    each entry.  Tokens of the first page before ``pos0[e]`` are kept; what the page held from there on
+    is not counted on any more."""
+    pages, heads, dh = _check("kv8_write", k_cache, v_cache, k_scale, v_scale, page_table, pos0,
+                              row0, max_rows)
+    k = _rows("kv8_write", k, heads * dh, k_cache)
+    v = _rows("kv8_write", v, heads * dh, k_cache)
+    if k.shape[0] != v.shape[0]:
+        raise ValueError(f"kv8_write: {k.shape[0]} rows of keys, {v.shape[0]} of values")
+    n, rows = page_table.shape[0], k.shape[0]
+    if row0 is None and n > rows:
+        raise ValueError(f"kv8_write: {n} entries, {rows} rows")
+    if n == 0 or rows == 0:
+        return
+    if k.is_cuda:
+        with torch.cuda.device(k.device):
+            rc = _lib.lib().cb_kv8_write(
+                _lib.ptr(k), _lib.ptr(v), k.stride(0), v.stride(0), _lib.ptr(k_cache),
+                _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale), _lib.ptr(page_table),
+                page_table.shape[1], pages, heads, dh, int(k_cache.dtype != torch.int8),
+                _lib.ptr(row0), _lib.ptr(pos0), n, rows, max_rows,
+                _lib.ptr(_lib.status_buffer(k.device)), _lib.stream_ptr())
+        _lib.check_rc(rc, "cb_kv8_write")
+        return
+    dtype = k_cache.dtype
+    for e, r0, cnt in _spans(n, row0, rows, max_rows):
+        at = int(pos0[e])
+        for lp in range(at // PAGE, (at + cnt - 1) // PAGE + 1):
+            page = _cpu_page(page_table, e, lp, pages)
+            lo, hi = max(0, at - lp * PAGE), min(PAGE, at + cnt - lp * PAGE)
+            r = r0 + lp * PAGE + lo - at
+            for x, codes, scale, keys in ((k, k_cache, k_scale, True), (v, v_cache, v_scale, False)):
+                new = x[r:r + hi - lo].float().view(hi - lo, heads, dh).transpose(0, 1)
+                amax = new.abs().amax((1, 2))
+                bad = ~torch.isfinite(amax)
+                ex = _exponent(torch.where(bad, torch.zeros_like(amax), amax), dtype)
+                old = _block(codes[page], keys)
+                if lo:
+                    bad = bad | torch.isnan(scale[page])
+                    was = torch.frexp(torch.nan_to_num(scale[page], 1.0))[1] - 1
+                    ex = torch.maximum(ex, was)
+                    shift = torch.where(bad, torch.zeros_like(ex), was - ex)
+                    kept = torch.ldexp(old[:, :lo], shift[:, None, None])
+                    old[:, :lo] = _encode(kept, dtype).float()
+                y = torch.where(bad[:, None, None], torch.zeros_like(new), torch.ldexp(new, -ex[:, None, None]))
+                old[:, lo:hi] = _encode(y, dtype).float()
+                c = _encode(old, dtype)
+                if keys:
+                    codes[page] = c.view(torch.int8).view(heads, PAGE, dh // 64, 64).transpose(1, 2).view(dtype)
+                else:
+                    codes[page] = c.view(torch.int8).transpose(1, 2).contiguous().view(dtype)
+                one = torch.ldexp(torch.ones(heads), ex)
+                scale[page] = torch.where(bad, torch.full_like(one, math.nan), one)
+
+
+def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+             v_scale: torch.Tensor, page_table: torch.Tensor, pos0: torch.Tensor,
+             row0: torch.Tensor, rows: int, max_rows: int,
+             dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The stored keys and values of positions ``pos0[e]`` and on as ``[rows, heads * dh]`` (``dtype``;
+    bf16 on a GPU, where it holds every stored value exactly).  ``rows`` is ``row0[n]``, known on the
+    host; rows that no entry owns are not set."""
+    pages, heads, dh = _check("kv8_read", k_cache, v_cache, k_scale, v_scale, page_table, pos0,
+                              row0, max_rows)
+    if row0 is None or rows < 0:
+        raise ValueError("kv8_read: needs row0 and the number of rows")
+    n = page_table.shape[0]
+    if k_cache.is_cuda:
+        if dtype != torch.bfloat16:
+            raise ValueError(f"kv8_read: the kernels give bf16, not {dtype}")
+        out = torch.empty((2, rows, heads * dh), dtype=dtype, device=k_cache.device)
+        if n and rows:
+            with torch.cuda.device(k_cache.device):
+                rc = _lib.lib().cb_kv8_read(
+                    _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale),
+                    _lib.ptr(page_table), page_table.shape[1], pages, heads, dh,
+                    int(k_cache.dtype != torch.int8), _lib.ptr(row0), _lib.ptr(pos0), n, rows,
+                    max_rows, _lib.ptr(out[0]), _lib.ptr(out[1]), heads * dh,
+                    _lib.ptr(_lib.status_buffer(k_cache.device)), _lib.stream_ptr())
+            _lib.check_rc(rc, "cb_kv8_read")
+        return out[0], out[1]
+    out = torch.zeros((2, rows, heads * dh), dtype=dtype)
+    for e, r0, cnt in _spans(n, row0, rows, max_rows):
+        at = int(pos0[e])
+        for lp in range(at // PAGE, (at + cnt - 1) // PAGE + 1):
+            page = _cpu_page(page_table, e, lp, pages)
+            lo, hi = max(0, at - lp * PAGE), min(PAGE, at + cnt - lp * PAGE)
+            r = r0 + lp * PAGE + lo - at
+            for o, codes, scale, keys in ((out[0], k_cache, k_scale, True),
+                                          (out[1], v_cache, v_scale, False)):
+                x = _values(codes, scale, page, keys)[:, lo:hi]
+                o[r:r + hi - lo] = x.transpose(0, 1).reshape(hi - lo, -1).to(dtype)
+    return out[0], out[1]
+
+
+def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
+                  ctx_len: torch.Tensor, nh: int, row0: Optional[torch.Tensor] = None,
+                  max_rows: int = 1, scale: Optional[float] = None) -> torch.Tensor:
+    """``q [rows, nh * dh]`` -> ``[rows, nh * dh]``.  Entry ``e`` holds ``ctx_len[e]`` tokens, its rows
+    are the last of them and every row sees the tokens up to itself; a row that sees none gets zeros, and
+    so do rows that no entry owns.  Query head ``h`` reads cache head ``h // (nh // heads)``; ``scale``
+    defaults to ``1 / sqrt(dh)``."""
+    pages, heads, dh = _check("kv8_attention", k_cache, v_cache, k_scale, v_scale, page_table,
+                              ctx_len, row0, max_rows)
+    if nh < 1 or nh % heads:
+        raise ValueError(f"kv8_attention: {nh} query heads over {heads}")
+    q = _rows("kv8_attention", q, nh * dh, k_cache)
+    n, rows = page_table.shape[0], q.shape[0]
+    if row0 is None and n > rows:
+        raise ValueError(f"kv8_attention: {n} entries, {rows} rows")
+    scale = scale if scale is not None else 1.0 / math.sqrt(dh)
+    if q.is_cuda:
+        whole = row0 is None and n == rows           # every row is written
+        out = (torch.empty if whole else torch.zeros)((rows, nh * dh), dtype=torch.bfloat16,
+                                                      device=q.device)
+        if n == 0 or rows == 0:
+            return out
+        with torch.cuda.device(q.device):
+            rc = _lib.lib().cb_kv8_attn(
+                _lib.ptr(q), q.stride(0), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale),
+                _lib.ptr(v_scale), _lib.ptr(page_table), page_table.shape[1], pages, heads, dh,
+                int(k_cache.dtype != torch.int8), _lib.ptr(ctx_len), _lib.ptr(row0), n, rows,
+                max_rows, nh, ctypes.c_float(scale), _lib.ptr(out), out.stride(0),
+                _lib.ptr(_lib.status_buffer(q.device)), _lib.stream_ptr())
+        _lib.check_rc(rc, "cb_kv8_attn")
+        return out
+    out = torch.zeros((rows, nh * dh), dtype=q.dtype)
+    g = nh // heads
+    for e, r0, cnt in _spans(n, row0, rows, max_rows):
+        c = int(ctx_len[e])
+        if c < 1:
+            continue
+        ids = [_cpu_page(page_table, e, lp, pages) for lp in range((c + PAGE - 1) // PAGE)]
+        K = torch.cat([_values(k_cache, k_scale, p, True) for p in ids], 1)[:, :c]
+        V = torch.cat([_values(v_cache, v_scale, p, False) for p in ids], 1)[:, :c]
+        x = q[r0:r0 + cnt].float().view(cnt, heads, g, dh)
+        s = torch.einsum("rhgd,hcd->hgrc", x, K) * scale
+        seen = torch.arange(c)[None] <= (c - cnt + torch.arange(cnt))[:, None]       # [rows, c]
+        # values a row does not see stay out of its sum, whatever they are
+        w = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        w = torch.where(seen, w, torch.zeros_like(w))
+        o = torch.einsum("hgrc,hcd->rhgd", w, V)
+        o = torch.where(seen.any(-1)[:, None, None, None], o, torch.zeros_like(o))
+        out[r0:r0 + cnt] = o.reshape(cnt, -1).to(q.dtype)
+    return out

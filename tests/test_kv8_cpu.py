@@ -1,0 +1,102 @@
+"""The 8-bit cache on the CPU (the restatement of its kernels) against its definition in 64 bits,
+and the calls that are refused."""
+import math
+
+import pytest
+import torch
+
+from coeus_b200.ops import kv8
+from kv8_cases import Case, i32
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_write_and_read(kind, dh):
+    c = Case(kind, 2, dh, [70, 200, 5])
+    c.write([0, 0, 0], [64, 130, 0])
+    c.write([64, 130, 0], [1, 1, 1])                       # a new page, the inside of one, the start
+    c.write([65, 131, 1], [1, 1, 1], sizes=[9.0, 40.0, 0.01])     # scales grow, or do not
+    c.write([66, 132, 2], [4, 68, 3], sizes=[100.0, 1.0, 1.0])
+    c.check_read([0, 0, 0], [70, 200, 5])
+    c.check_read([63, 129, 4], [3, 70, 1])
+
+
+def test_codes_use_the_range_and_ties_go_to_even():
+    c = Case("int8", 1, 64, [1])
+    k = torch.zeros(1, 64)
+    k[0, :4] = torch.tensor([127.0, 0.5, 1.5, -2.5])
+    kv8.kv8_write(k, k, *c.c, c.table, i32([0]))
+    page = int(c.table[0, 0])
+    assert float(c.c[2][page, 0]) == 1.0
+    assert c.c[0][page, 0, 0, 0, :4].tolist() == [127, 0, 2, -2]
+    assert c.c[1][page, 0, :4, 0].tolist() == [127, 0, 2, -2]
+    k[0, 0] = 127.5
+    kv8.kv8_write(k, k, *c.c, c.table, i32([0]))
+    assert float(c.c[2][page, 0]) == 2.0
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_not_a_number_makes_its_block_one(kind):
+    c = Case(kind, 2, 64, [130])
+
+    def edit(k, v):
+        k[3, 5] = math.inf                                 # page 0, head 0, keys
+        v[70, 64 + 2] = math.nan                           # page 1, head 1, values
+    c.write([0], [130], edit=edit)
+    c.check_read([0], [130])
+    k, v = c.read([0], [130])
+    assert torch.isnan(k[:64, :64]).all() and not torch.isnan(k[64:]).any()
+    assert torch.isnan(v[64:128, 64:]).all() and not torch.isnan(v[:64]).any()
+    c.write([0], [130])                                    # from its first token on a page is new
+    c.check_read([0], [130])
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("nh,heads,dh", [(2, 2, 64), (6, 2, 64), (4, 1, 128)])
+def test_attention(kind, nh, heads, dh):
+    c = Case(kind, heads, dh, [1, 64, 130, 3])
+    c.write([0] * 4, [1, 64, 130, 3])
+    c.check_attend([1, 64, 130, 3], [1, 1, 1, 1], nh)
+    c.check_attend([1, 64, 130, 3], [1, 0, 70, 5], nh)     # the last entry's first rows see nothing
+    c.check_attend([0, 64, 129, 0], [1, 3, 2, 1], nh, scale=0.3)
+
+
+def test_refusals():
+    c = Case("int8", 2, 64, [70, 3])
+    k, v, ks, vs = c.c
+    x = torch.zeros(2, 128)
+    pos = i32([0, 0])
+    ok = (x, x, k, v, ks, vs, c.table, pos)
+
+    def refused(**kw):
+        names = ["k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "page_table", "pos0"]
+        args = dict(zip(names, ok), **kw)
+        with pytest.raises(ValueError):
+            kv8.kv8_write(**args)
+    refused(k=torch.zeros(2, 64))
+    refused(k=torch.zeros(3, 128))
+    refused(k=torch.zeros(1, 128), v=torch.zeros(1, 128))
+    refused(v_cache=v[:, :1])
+    refused(v_cache=v.view(torch.float8_e4m3fn))
+    refused(k_cache=k.float())
+    refused(k_scale=ks.double())
+    refused(page_table=c.table.long())
+    refused(page_table=c.table.t().contiguous().t())
+    refused(pos0=i32([0]))
+    refused(pos0=pos.long())
+    refused(max_rows=2)
+    refused(row0=i32([0, 1]))
+    refused(row0=i32([0, 1, 2]), max_rows=0)
+    refused(row0=i32([0, 2, 2]), max_rows=1)
+    refused(row0=i32([0, 1, 3]), max_rows=2)
+    refused(pos0=i32([0, 64]))                             # no second page
+    with pytest.raises(ValueError):
+        kv8.kv8_attention(torch.zeros(2, 192), k, v, ks, vs, c.table, pos, 3)
+    with pytest.raises(ValueError):
+        kv8.kv8_attention(torch.zeros(1, 128), k, v, ks, vs, c.table, pos, 2)
+    with pytest.raises(ValueError):
+        kv8.kv8_alloc(4, 2, 96, "int8", "cpu")
+    with pytest.raises(ValueError):
+        kv8.kv8_alloc(4, 2, 64, "fp4", "cpu")
+    with pytest.raises(ValueError):
+        kv8.kv8_read(k, v, ks, vs, c.table, pos, None, 2, 1)

@@ -1,0 +1,244 @@
+"""The kernels of the 8-bit cache against its definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from coeus_b200.ops import _lib, kv8
+from kv8_cases import Case, i32, starts
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def status():
+    torch.cuda.synchronize()
+    s = _lib.status_buffer(torch.device("cuda", 0))
+    code = int(s[0])
+    s.zero_()
+    return code
+
+
+KINDS = ["int8", "e4m3"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,dh", [(1, 64), (3, 64), (2, 128)])
+def test_write_and_read(kind, heads, dh):
+    c = Case(kind, heads, dh, [70, 300, 5, 64], DEV)
+    c.write([0] * 4, [64, 130, 0, 64])
+    c.write([64, 130, 0, 0], [1, 1, 1, 1])
+    c.write([65, 131, 1, 1], [1, 1, 1, 1], sizes=[9.0, 40.0, 0.01, 1e4])
+    c.write([66, 132, 2, 2], [4, 168, 3, 62], sizes=[100.0, 1.0, 1.0, 1e-3])
+    c.check_read([0] * 4, [70, 300, 5, 64])
+    c.check_read([63, 129, 4, 0], [3, 70, 1, 0])
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_write_extremes(kind):
+    """Zeros, the smallest and largest magnitudes, values next to where the scale steps."""
+    c = Case(kind, 2, 64, [64, 64, 64, 64], DEV)
+
+    def edit(k, v):
+        k[0:3] = 0.0
+        k[3:6] *= 1e-38
+        k[6:9] = k[6:9].float().mul(1e38).clamp(-3e38, 3e38).bfloat16()
+        k[9:12] = 0.0
+        k[9, 0], k[10, 64], k[11, 70] = 127.0, 127.5, -448.0
+        v[9:12] = 0.0
+        v[9, 0], v[10, 64], v[11, 70] = 448.0, 450.0, -896.0
+    c.write([0] * 4, [3, 3, 3, 3], edit=edit)
+    c.check_read([0] * 4, [3, 3, 3, 3])
+    c.write([3] * 4, [2, 2, 2, 2])
+    c.check_read([0] * 4, [5, 5, 5, 5])
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_not_a_number_makes_its_block_one(kind):
+    c = Case(kind, 2, 64, [130], DEV)
+
+    def edit(k, v):
+        k[3, 5] = math.inf
+        v[70, 64 + 2] = math.nan
+    c.write([0], [128], edit=edit)
+    c.write([128], [1])
+    c.check_read([0], [129])
+    # head 0 reads NaN keys, head 1 NaN values, but not with a context that ends before them
+    o = c.check_attend([129], [1], 2)
+    assert torch.isnan(o).all()
+    o = c.check_attend([64], [3], 2)
+    assert torch.isnan(o[:, :64]).all() and not torch.isnan(o[:, 64:]).any()
+    # a row in front of the block is not touched by it
+    o = c.check_attend([66], [4], 2)
+    assert not torch.isnan(o[0:2, 64:]).any() and torch.isnan(o[2:, 64:]).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,heads,dh", [(2, 2, 64), (16, 16, 64), (6, 2, 64), (7, 1, 128), (8, 1, 128),
+                                         (9, 1, 64), (16, 1, 128), (24, 2, 128), (40, 1, 64)])
+def test_attention_one_row(kind, nh, heads, dh):
+    lens = [1, 63, 64, 65, 333, 3]
+    c = Case(kind, heads, dh, lens, DEV)
+    c.write([0] * 6, lens)
+    c.check_attend(lens, [1] * 6, nh)
+    c.check_attend([0, 62, 1, 64, 300, 0], [1] * 6, nh, scale=0.2)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,heads,dh", [(2, 2, 64), (3, 1, 128), (8, 2, 128), (5, 1, 64)])
+@pytest.mark.parametrize("rows", [[2, 0, 9, 1, 5], [1, 64, 17, 130, 40], [3, 3, 3, 3, 3]])
+def test_attention_several_rows(kind, nh, heads, dh, rows):
+    lens = [2, 64, 200, 131, 44]
+    c = Case(kind, heads, dh, lens, DEV)
+    c.write([0] * 5, lens)
+    c.check_attend(lens, rows, nh)
+    c.check_attend([1, 64, 199, 129, 0], rows, nh, max_rows=max(rows) + 70)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_long_context(kind):
+    n = 20000
+    c = Case(kind, 1, 128, [n, 64], DEV)
+    c.write([0, 0], [n, 64])
+    c.check_attend([n, 64], [1, 1], 4)
+    c.check_attend([n - 63, 10], [3, 2], 4, size=3.0)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_scales_apart(kind):
+    """Pages whose values differ by 2^30, and a row that only listens to the small ones."""
+    c = Case(kind, 1, 64, [192], DEV)
+    c.write([0], [64], sizes=[3e4])
+    c.write([64], [64], sizes=[3e-5])
+    c.write([128], [64])
+    c.check_attend([192], [1], 2, size=1e-4)
+    c.check_attend([128], [3], 2, size=3e-4)
+    # keys of the first page far below the others' scores
+    c = Case(kind, 1, 64, [128], DEV)
+
+    def edit(k, v):
+        k[:64] = -2.0
+        k[64:] = 2.0
+        v[:64] *= 2.0 ** 15
+        v[64:] *= 2.0 ** -15
+    c.write([0], [128], edit=edit)
+    q = torch.full((1, 64), 2.0, dtype=torch.bfloat16)
+    got = c.attend(q, [128], [1], 1).double().cpu()
+    want, spread = c.plain.attention(q, c.table, [128], [1], 1, 64 ** -0.5)
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_stale_codes_behind_the_context(kind):
+    """What the last page holds behind the context is never used, whatever it is."""
+    c = Case(kind, 1, 64, [70], DEV)
+    c.write([0], [70])
+    page = int(c.table[0, 1])
+    c.c[0].view(torch.int8)[page, 0, 0, 6:] = 127         # e4m3: NaN
+    c.c[1].view(torch.int8)[page, 0, :, 6:] = 127
+    c.check_attend([70], [1], 2)
+    c.check_attend([70], [10], 2)
+    c.check_attend([70], [40], 2)
+    assert status() == 0
+
+
+def test_layouts_streams_and_graphs():
+    c = Case("int8", 2, 64, [100, 130], DEV)
+    c.write([0, 0], [99, 129])
+    wide = torch.randn(2, 3 * 128 + 3, device=DEV).bfloat16()
+    k, v = wide[:, 1:129], wide[:, 129:257]               # neither aligned nor packed
+    kv8.kv8_write(k, v, *c.c, c.table.to(DEV), i32([99, 129], DEV))
+    c.plain.write(k.cpu(), v.cpu(), c.table, [99, 129], [1, 1])
+    c.check_read([60, 60], [40, 70])
+    q = wide[:, 200:328]
+    table, ctx = c.table.to(DEV), i32([100, 130], DEV)
+    want = kv8.kv8_attention(q, *c.c, table, ctx, 2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(kv8.kv8_attention(q, *c.c, table, ctx, 2), want)
+    torch.cuda.current_stream().wait_stream(side)
+    # two graphs over the same tensors, replayed in either order with changed inputs
+    pos = i32([99, 129], DEV)
+    k, v, q = k.contiguous(), v.contiguous(), q.contiguous()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            kv8.kv8_write(k, v, *c.c, table, pos)
+            out = kv8.kv8_attention(q, *c.c, table, ctx, 2)
+        graphs.append((g, out))
+    for g, out in graphs[::-1] + graphs:
+        for t in (k, v, q):
+            t.copy_(torch.randn_like(t))
+        g.replay()
+        c.plain.write(k.cpu(), v.cpu(), c.table, [99, 129], [1, 1])
+        want, spread = c.plain.attention(q.cpu(), c.table, [100, 130], [1, 1], 2, 0.125)
+        err = (out.double().cpu() - want).abs()
+        assert (err <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all()
+    assert status() == 0
+
+
+def test_repeated_calls_give_the_same_bits():
+    c = Case("e4m3", 2, 128, [5000, 40], DEV)
+    c.write([0, 0], [5000, 40])
+    q = torch.randn(2, 8 * 128, device=DEV).bfloat16()
+    outs = [c.attend(q, [5000, 40], [1, 1], 8) for _ in range(5)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    assert status() == 0
+
+
+def test_rows_without_entry_and_bad_entries():
+    """Rows behind the last entry are zero; an entry out of range is skipped and recorded, the
+    others are answered."""
+    c = Case("int8", 1, 64, [100, 40, 70], DEV)
+    c.write([0] * 3, [100, 40, 70])
+    q = torch.randn(9, 128, device=DEV).bfloat16()
+    table, ctx = c.table.to(DEV), i32([100, 40, 70], DEV)
+    row0 = i32([0, 2, 2, 5], DEV)
+    out = kv8.kv8_attention(q, *c.c, table, ctx, 2, row0=row0, max_rows=4)
+    assert (out[5:] == 0).all() and status() == 0
+    # more rows than max_rows: that entry is refused alone
+    bad = kv8.kv8_attention(q, *c.c, table, ctx, 2, row0=row0, max_rows=2)
+    assert torch.equal(bad[:2], out[:2]) and (bad[2:] == 0).all() and status() == 2
+    # rows past the tensor
+    bad = kv8.kv8_attention(q[:4], *c.c, table, ctx, 2, row0=row0, max_rows=4)
+    assert torch.equal(bad[:2], out[:2]) and (bad[2:] == 0).all() and status() == 2
+    # a page number that the cache does not have
+    wrong = table.clone()
+    wrong[2, 1] = 10 ** 6
+    bad = kv8.kv8_attention(q, *c.c, wrong, ctx, 2, row0=row0, max_rows=4)
+    assert torch.equal(bad[:2], out[:2]) and status() == 2
+    before = [t.clone() for t in c.c]
+    k = torch.randn(3, 64, device=DEV).bfloat16()
+    kv8.kv8_write(k, k, *c.c, wrong[2:], i32([70], DEV), row0=i32([0, 3], DEV), max_rows=3)
+    assert status() == 2
+    kv8.kv8_write(k, k, *c.c, table[2:], i32([-5], DEV), row0=i32([0, 3], DEV), max_rows=3)
+    assert status() == 2
+    kv8.kv8_write(k, k, *c.c, table[1:2], i32([400], DEV), row0=i32([0, 3], DEV), max_rows=3)
+    assert status() == 2
+    kv8.kv8_write(k, k, *c.c, table[1:2], i32([0], DEV), row0=i32([0, 9], DEV), max_rows=9)
+    assert status() == 2
+    for a, b in zip(before, c.c):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_gpu_refusals():
+    c = Case("int8", 1, 64, [3], DEV)
+    x = torch.zeros(1, 64, device=DEV)
+    with pytest.raises(ValueError):
+        kv8.kv8_write(x, x, *c.c, c.table.to(DEV), i32([0], DEV))
+    with pytest.raises(ValueError):
+        kv8.kv8_write(x.bfloat16(), x.bfloat16(), *c.c, c.table, i32([0], DEV))
+    with pytest.raises(ValueError):
+        kv8.kv8_attention(x.bfloat16().cpu(), *c.c, c.table.to(DEV), i32([1], DEV), 1)
+    with pytest.raises(ValueError):
+        kv8.kv8_read(*c.c, c.table.to(DEV), i32([0], DEV), i32([0, 1], DEV), 1, 1,
+                     dtype=torch.float32)

@@ -4,129 +4,690 @@
 //
 //   o = sum_t w_t v_t / sum_t w_t,  w_t = exp(scale q . k_t - max),  k_t = code 2^ek, v_t = code 2^ev
 //
-// One CTA per row and head; its warps take the pages in turn and are merged at the end.
+// The cache has to be streamed once, two bytes of it per key and channel, and everything else has to
+// hide behind that.  Work is cut into units of one page of one key/value head for one tile of eight query rows
+// (rows and heads that share the head).  A CTA is one warp that takes an equal run of units, whatever the lengths of
+// the sequences, and keeps its next pages coming with bulk copies (a page's keys and values are 64 dh bytes each); as
+// many CTAs as shared memory holds share an SM (dh 128: six) and know nothing of each other.  Warps of one CTA that
+// took the pages of a tile in turn and merged their parts waited for one another: 1.3 times the time.
+//
+// Both products are transposed, S^T = K Q^T and O^T = V^T P^T (mma m16n8k16 in fp16, fp32 sums), so that
+// the cached side is the operand of 16 rows and the few query rows are the eight columns.  Which
+// token or channel a row or column of a fragment stands for is free as long as both operands agree, and
+// is chosen so that every fragment of the cached side is consecutive bytes of a lane:
+//   keys     lane (g, c) holds channels 16c .. 16c + 15 of a 64-channel half; one of its four words per k-step
+//   tokens   row r of the eight of (step s, half u) is token 16 (r / 2) + 4 s + 2 u + r % 2, so that after
+//            the transposition of the weights (movmatrix) lane (g, c) has tokens 16c + 4s .. + 3: the
+//            word s of its 16 bytes of a row of values
+// Codes become fp16 exactly: int8 by setting the biased byte into the mantissa of 1024 and subtracting, e4m3
+// by its conversion.  Queries are fp16 after division by a power of two per row.  Weights enter the second product
+// as fp16 times 2^12: smaller than 2^-26 of the row's largest they start to lose bits, and less than 2^-36
+// of it is lost in all; the page's 2^ev is applied in fp32 to the sums of a page.
 #include "kv8.cuh"
 
 namespace cb {
+
+constexpr int KA_ROWS = 8;                        // query rows of a tile
+constexpr int KA_ENTRIES = 256;                   // of one launch
+constexpr int KA_SHARE = 2;                       // units a CTA takes at least
+constexpr int KA_EXTRA = 1;                       // what a tile costs beside its pages, in units
+constexpr int KA_BLOCK = 16;                      // units that are planned at a time
+constexpr int KA_RING = 4;                        // copies in a warp's ring: the keys and values of two pages
+constexpr int KA_PLACES = 6, KA_PLACES64 = 11;    // CTAs that share an SM, by its shared memory: dh 128, 64
+constexpr float KA_SHIFT = 12.f;                  // weights are held times 2^12
+
+struct Kv8Desc {           // the tile that a CTA's run of units starts in
+  int lo, hi, share, units;
+  int entry, head, tile, pad;
+};
 
 struct Kv8Attn {
   Kv8Cache c;
   const __nv_bfloat16* q;  // [rows, ldq]
   __nv_bfloat16* out;      // [rows, ldo]
-  int ldq, ldo, heads;
+  int ldq, ldo, group;     // query heads per key/value head
   const int* ctx;          // [entries]
-  const int* row0;         // [entries + 1] or null: entry e has row e alone
-  int rows, most;
+  const int* row0;         // [entries + 1] or null: entry e has row first + e alone
+  int first, n, rows, most;
   float scale_log2;
+  float* part_o;           // [CTAs, 2, KA_ROWS, dh]
+  float* part_ml;          // [CTAs, 2, KA_ROWS, 2]
+  Kv8Desc* desc;           // [CTAs]
   int* status;
 };
 
-constexpr int KA_WARPS = 4;
+// Four codes to two pairs of fp16.
+template <int KIND>
+__device__ __forceinline__ void kv8_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (KIND == KV8_INT8) {
+    const uint32_t x = w ^ 0x80808080u;                       // code + 128
+    lo = __byte_perm(x, 0x64646464u, 0x4140);                 // 1024 + that
+    hi = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+    const __half2 p = __hsub2(*reinterpret_cast<__half2*>(&lo), off), q = __hsub2(*reinterpret_cast<__half2*>(&hi), off);
+    lo = *reinterpret_cast<const uint32_t*>(&p);
+    hi = *reinterpret_cast<const uint32_t*>(&q);
+  } else {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Wait for a phase, with a limit; the clock is asked only after many tries have failed.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  const uint32_t at = smem_u32(bar);
+  uint64_t began = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(at, parity)) return true;
+    if (n % 256u == 0u) {
+      if (*abort_flag) return false;
+      const uint64_t now = globaltimer_ns();
+      if (began == 0) began = now;
+      else if (now - began > CB_WAIT_LIMIT_NS) {
+        *abort_flag = 1u;
+        return false;
+      }
+    }
+  }
+}
+
+// What one part of a softmax counts against the whole: its maximum m and sum l, the largest maximum.
+// A part without keys has m = -inf and l = 0; one whose scores are NaN has l = NaN, which stays.
+__device__ __forceinline__ float part_weight(float m, float l, float gm) {
+  if (m == -INFINITY) return l == 0.f ? 0.f : 1.f;
+  return fast_exp2(m - gm);
+}
+
+// Entry of a launch: rows and context as they are used; -1 rows if something is out of range.
+struct Kv8Entry {
+  int first, rows, ctx;
+};
+__device__ __forceinline__ Kv8Entry kv8_entry(const Kv8Attn& a, int e) {
+  Kv8Entry x;
+  x.first = a.row0 != nullptr ? a.row0[e] : a.first + e;
+  x.rows = a.row0 != nullptr ? a.row0[e + 1] - x.first : 1;
+  x.ctx = max(0, a.ctx[e]);
+  if (x.rows <= 0) x.rows = 0;
+  else if (x.rows > a.most || x.first < 0 || x.first + x.rows > a.rows) x.rows = -1;
+  return x;
+}
+
+// A unit as it is planned: a page of a tile, and the tile's share of the CTA's units (counted from 0).
+struct Kv8Unit {
+  int flags;               // UNIT_*
+  int page, p;             // page of the cache, of the sequence
+  int first, rows, ctx;    // the entry's
+  int head, tile;
+  float ks, vs;
+};
+// a page (and not a tile's extra); with keys that count; the tile's first page here; its last; all of the tile is here;
+// it is the CTA's first tile
+enum : int { UNIT_PAGE = 1, UNIT_LIVE = 2, UNIT_BEGIN = 4, UNIT_LAST = 8, UNIT_WHOLE = 16, UNIT_FIRST = 32 };
+
+template <int DH>
+struct Kv8Smem {
+  static constexpr int SLOT = KV8_PAGE * DH;                    // bytes of a page's keys, or of its values
+  static constexpr int BYTES = KA_RING * (SLOT + 8) + (KA_ENTRIES + 1) * 4 + 2 * KA_BLOCK * static_cast<int>(sizeof(Kv8Unit)) + 32;
+};
 
 template <int KIND, int DH>
-__global__ void __launch_bounds__(KA_WARPS * 32) kv8_attn_kernel(const Kv8Attn a) {
-  __shared__ float sq[DH], sw[KA_WARPS][KV8_PAGE], sm[KA_WARPS], sl[KA_WARPS], so[KA_WARPS][DH];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int b = blockIdx.x;
-  const int h = b % a.heads;
-  b /= a.heads;
-  const int i = b % a.most, e = b / a.most;
-  const int first = a.row0 != nullptr ? a.row0[e] : e;
-  const int n = a.row0 != nullptr ? a.row0[e + 1] - first : 1;
-  if (i >= n) return;
-  if (n > a.most || first < 0 || first + n > a.rows) {
-    record_status(a.status, ST_BOUNDS, e);
-    return;
-  }
-  const int seen = a.ctx[e] - n + i + 1;
-  const int hk = h / (a.heads / a.c.heads);
-  for (int d = threadIdx.x; d < DH; d += KA_WARPS * 32)
-    sq[d] = __bfloat162float(a.q[static_cast<size_t>(first + i) * a.ldq + h * DH + d]) * a.scale_log2;
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[DH / 32];
-#pragma unroll
-  for (int x = 0; x < DH / 32; ++x) o[x] = 0.f;
-  for (int p = warp; p * KV8_PAGE < seen; p += KA_WARPS) {
-    const int page = kv8_page(a.c, e, p, a.status, e);
-    if (page < 0) continue;
-    const size_t cell = static_cast<size_t>(page) * a.c.heads + hk;
-    const uint8_t* kb = a.c.k + cell * (KV8_PAGE * DH);
-    const uint8_t* vb = a.c.v + cell * (KV8_PAGE * DH);
-    const float ks = a.c.k_scale[cell], vs = a.c.v_scale[cell];
-    float s[2], mx = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int t = lane + 32 * x;
-      float dot = 0.f;
-      for (int d = 0; d < DH; ++d) dot += sq[d] * kv8_value<KIND>(kb[(d / 64 * KV8_PAGE + t) * 64 + d % 64]);
-      s[x] = p * KV8_PAGE + t < seen ? dot * ks : -INFINITY;
-      mx = fmaxf(mx, s[x]);
-    }
-    const float mn = fmaxf(m, warp_max(mx)), c = exp2f(m - mn);
-    m = mn;
-    l *= c;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float w = exp2f(s[x] - mn);
-      l += w;
-      sw[warp][lane + 32 * x] = w;
-    }
-    __syncwarp();
-    const int nt = min(KV8_PAGE, seen - p * KV8_PAGE);
-#pragma unroll
-    for (int x = 0; x < DH / 32; ++x) {
-      float acc = 0.f;
-      for (int t = 0; t < nt; ++t) acc += sw[warp][t] * kv8_value<KIND>(vb[(lane + 32 * x) * KV8_PAGE + t]);
-      o[x] = o[x] * c + acc * vs;
-    }
-    __syncwarp();
-  }
-  l = warp_sum(l);
+__global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv8Attn a) {
+  using S = Kv8Smem<DH>;
+  constexpr int QR = KA_ROWS, RING = KA_RING, AHEAD = RING / 2;                 // pages ahead of the one that is computed
+  extern __shared__ __align__(128) unsigned char smem[];
+  unsigned char* ring = smem;                                                   // [RING][SLOT]
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + RING * S::SLOT);          // [RING]: the copy is there
+  int* prefix = reinterpret_cast<int*>(full + RING);                            // [KA_ENTRIES + 1]: units before every entry
+  Kv8Unit* book = reinterpret_cast<Kv8Unit*>((reinterpret_cast<uintptr_t>(prefix + KA_ENTRIES + 1) + 15) & ~uintptr_t(15));  // [2][KA_BLOCK]
+  __shared__ volatile uint32_t abort_flag;
+  const int lane = threadIdx.x, nkv = a.c.heads;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- the plan: units before every entry
   if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+    abort_flag = 0u;
+    prefix[0] = 0;
+    for (int i = 0; i < RING; ++i) mbar_init(smem_u32(full + i), 1);
+    mbar_fence_init();
   }
+  auto entry_of = [&](int e) {                                  // rows 0: nothing to do
+    Kv8Entry x = kv8_entry(a, e);
+    x.rows = max(x.rows, 0);
+    x.ctx = min(x.ctx, a.c.max_pages * KV8_PAGE);
+    return x;
+  };
+  int units = 0;
+#pragma unroll 4
+  for (int e0 = 0; e0 < a.n; e0 += 32) {
+    const int e = e0 + lane;
+    int s = 0;
+    if (e < a.n) {
+      const Kv8Entry x = entry_of(e);
+      if (blockIdx.x == 0 && (kv8_entry(a, e).rows < 0 || a.ctx[e] > a.c.max_pages * KV8_PAGE)) record_status(a.status, ST_BOUNDS, e);
+      if (x.ctx > 0) s = (x.rows * a.group + QR - 1) / QR * ((x.ctx + KV8_PAGE - 1) / KV8_PAGE + KA_EXTRA) * nkv;
+    }
 #pragma unroll
-  for (int x = 0; x < DH / 32; ++x) so[warp][lane + 32 * x] = o[x];
-  __syncthreads();
-  float gm = -INFINITY, gl = 0.f;
-  for (int w = 0; w < KA_WARPS; ++w) gm = fmaxf(gm, sm[w]);
-  for (int w = 0; w < KA_WARPS; ++w) gl += sl[w] == 0.f ? 0.f : sl[w] * exp2f(sm[w] - gm);   // NaN stays
-  for (int d = threadIdx.x; d < DH; d += KA_WARPS * 32) {
-    float v = 0.f;
-    for (int w = 0; w < KA_WARPS; ++w) v += sm[w] == -INFINITY ? 0.f : so[w][d] * exp2f(sm[w] - gm);
-    a.out[static_cast<size_t>(first + i) * a.ldo + h * DH + d] = __float2bfloat16(seen > 0 ? v / gl : 0.f);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += t;
+    }
+    if (e < a.n) prefix[e + 1] = units + s;
+    units += __shfl_sync(0xffffffffu, s, 31);
   }
+  __syncwarp();
+  const int share = max((units - 1) / static_cast<int>(gridDim.x) + 1, KA_SHARE);
+  const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(share) * blockIdx.x));
+  const int u1 = min(units - u0, share) + u0, n_units = u1 - u0;
+
+  struct Where {           // a unit's tile
+    int e, hk, tile, pages;
+    int lo;                // its first unit
+    Kv8Entry x;
+  };
+  auto locate = [&](int u) {
+    int lo = 0, hi = a.n;                                       // prefix[lo] <= u < prefix[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    Where w;
+    w.e = lo;
+    w.x = entry_of(lo);
+    w.pages = (w.x.ctx + KV8_PAGE - 1) / KV8_PAGE;
+    const int tiles = (w.x.rows * a.group + QR - 1) / QR, t = (u - prefix[lo]) / (w.pages + KA_EXTRA);
+    w.hk = t / tiles;
+    w.tile = t % tiles;
+    w.lo = prefix[lo] + t * (w.pages + KA_EXTRA);
+    return w;
+  };
+  if (lane == 0) {
+    Kv8Desc d{u0, u0, share, units, 0, 0, 0, 0};
+    if (n_units > 0) {
+      const Where w = locate(u0);
+      d.lo = w.lo;
+      d.hi = w.lo + w.pages;
+      d.entry = w.e;
+      d.head = w.hk;
+      d.tile = w.tile;
+    }
+    a.desc[blockIdx.x] = d;
+  }
+  // ---- entries without keys: their rows are zero
+  for (int e = blockIdx.x; e < a.n; e += gridDim.x) {
+    const Kv8Entry x = entry_of(e);
+    if (x.ctx == 0)
+      for (int r = 0; r < x.rows; ++r)
+        for (int i = lane; i < a.group * nkv * DH; i += 32) a.out[static_cast<size_t>(x.first + r) * a.ldo + i] = __float2bfloat16(0.f);
+  }
+
+  const int g = lane >> 2, c = lane & 3;
+  // Units are planned KA_BLOCK at a time, one a lane, while those before them run: what the page table and the scales
+  // take to answer is hidden.
+  Kv8Unit x;
+  auto plan_page = [&](int block) {                             // place of the lane's unit, its page asked for
+    const int j = block * KA_BLOCK + lane;
+    x.flags = 0;
+    if (j >= n_units || lane >= KA_BLOCK) return;
+    const Where w = locate(u0 + j);
+    x.p = u0 + j - w.lo;
+    if (x.p >= w.pages) return;
+    x.flags = UNIT_PAGE;
+    x.first = w.x.first;
+    x.rows = w.x.rows;
+    x.ctx = w.x.ctx;
+    x.head = w.hk;
+    x.tile = w.tile;
+    if (x.p == 0 || j == 0) x.flags |= UNIT_BEGIN;
+    if (x.p == w.pages - 1 || j == n_units - 1) x.flags |= UNIT_LAST;
+    if (w.lo >= u0 && w.lo + w.pages <= u1) x.flags |= UNIT_WHOLE;
+    if (w.lo <= u0) x.flags |= UNIT_FIRST;
+    // a page behind what the last row of the tile sees is not read
+    const int last = min(w.x.rows - 1, (w.tile * QR + QR - 1) / a.group);
+    if (x.p * KV8_PAGE < w.x.ctx - w.x.rows + last + 1) {
+      x.flags |= UNIT_LIVE;
+      x.page = a.c.page_table[static_cast<size_t>(w.e) * a.c.max_pages + x.p];
+    }
+  };
+  auto plan_check = [&]() {                                     // the page is known
+    if ((x.flags & UNIT_LIVE) && (x.page < 0 || x.page >= a.c.num_pages)) {
+      record_status(a.status, ST_BOUNDS, x.first);
+      x.flags &= ~UNIT_LIVE;
+    }
+  };
+  auto plan_scale = [&]() {                                     // its scales are asked for
+    if (!(x.flags & UNIT_LIVE)) return;
+    const size_t cell = static_cast<size_t>(x.page) * nkv + x.head;
+    x.ks = a.c.k_scale[cell];
+    x.vs = a.c.v_scale[cell];
+  };
+  auto plan_done = [&](int block) {
+    if (lane < KA_BLOCK) book[(block & 1) * KA_BLOCK + lane] = x;
+    __syncwarp();
+  };
+  auto unit_at = [&](int i) -> const Kv8Unit& { return book[i % (2 * KA_BLOCK)]; };
+  int asked = 0, done = 0;                                      // pages copied, computed
+  bool dead = false;
+  auto ask = [&](int i) {                                       // the copies of unit i
+    const Kv8Unit& y = unit_at(i);
+    if (!(y.flags & UNIT_LIVE)) return;
+    if (lane == 0) {
+      const size_t at = (static_cast<size_t>(y.page) * nkv + y.head) * S::SLOT;
+      const int k = 2 * asked % RING, v = k + 1;
+      mbar_arrive_expect_tx(smem_u32(full + k), S::SLOT);
+      bulk_load_g2s(smem_u32(ring + k * S::SLOT), a.c.k + at, S::SLOT, smem_u32(full + k));
+      mbar_arrive_expect_tx(smem_u32(full + v), S::SLOT);
+      bulk_load_g2s(smem_u32(ring + v * S::SLOT), a.c.v + at, S::SLOT, smem_u32(full + v));
+    }
+    ++asked;
+  };
+  auto failed = [&]() {
+    dead = true;
+    if (lane == 0) record_status(a.status, ST_WAIT_TIMEOUT, blockIdx.x);
+  };
+  plan_page(0);
+  plan_check();
+  plan_done(0);
+  for (int i = 0; i < min(AHEAD, n_units); ++i) ask(i);          // the first copies do not wait for the scales
+  plan_scale();
+  plan_done(0);
+  uint32_t qf[DH / 64][4][2];
+  float f[2], o[DH / 16][4], m[2], l[2];                         // columns 2c and 2c + 1; f: score per product
+  int seen[2], least_seen = 0, all_seen = 0;
+  for (int i = 0; i < n_units; ++i) {
+    if ((i / KA_BLOCK + 1) * KA_BLOCK < n_units) {
+      if (i % KA_BLOCK == 0) plan_page(i / KA_BLOCK + 1);
+      else if (i % KA_BLOCK == 5) { plan_check(); plan_scale(); }
+      else if (i % KA_BLOCK == 10) plan_done(i / KA_BLOCK + 1);
+    }
+    const Kv8Unit un = unit_at(i);
+    if (un.flags & UNIT_PAGE) {
+    const bool live = un.flags & UNIT_LIVE;
+    const int sk = 2 * done % RING, sv = sk + 1;
+    const uint32_t phase = 2 * done / RING & 1;
+    const float ks = un.ks, vs = un.vs;
+    const int rows = un.rows, ctx = un.ctx, first = un.first;
+    const int total = rows * a.group;                            // rows of all tiles of this head
+    if (un.flags & UNIT_BEGIN) {
+      // ---- a new tile: its queries; lane (g, c) has row g, channels 16c .. of every half
+      const int r = un.tile * QR + g;
+      uint4 x[DH / 64][2];
+      float top = 0.f;
+#pragma unroll
+      for (int h = 0; h < DH / 64; ++h)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          x[h][y] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < total) {
+            const __nv_bfloat16* src = a.q + static_cast<size_t>(first + r / a.group) * a.ldq +
+                                       (un.head * a.group + r % a.group) * DH + h * 64 + c * 16 + y * 8;
+            x[h][y] = __ldg(reinterpret_cast<const uint4*>(src));
+          }
+        }
+#pragma unroll
+      for (int h = 0; h < DH / 64; ++h)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t* v = reinterpret_cast<const uint32_t*>(&x[h][y]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 b = unpack_bf16x2(v[i]);
+            top = fmaxf(top, fmaxf(fabsf(b.x), fabsf(b.y)));
+          }
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^k is the binade of the row's largest number; a row of zeros or infinities stays as it is
+      const int k = top > 0.f && top < INFINITY ? max(min((__float_as_int(top) >> 23) - 127, 126), -126) : 0;
+      const float down = pow2(-k), up = pow2(k) * a.scale_log2;
+#pragma unroll
+      for (int h = 0; h < DH / 64; ++h)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t* v = reinterpret_cast<const uint32_t*>(&x[h][y]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {                          // channels 16c + 8y + 2i, + 1
+            const float2 b = unpack_bf16x2(v[i]);
+            qf[h][2 * y + i / 2][i % 2] = half2_bits(b.x * down, b.y * down);
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f[i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
+        seen[i] = ctx - rows + min(un.tile * QR + 2 * c + i, total - 1) / a.group + 1;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+      }
+      least_seen = ctx - rows + (un.tile * QR) / a.group + 1;
+      all_seen = ctx - rows + min(rows - 1, (un.tile * QR + QR - 1) / a.group) + 1;
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i)
+#pragma unroll
+        for (int x2 = 0; x2 < 4; ++x2) o[i][x2] = 0.f;
+    }
+    if (live && !dead && !wait_phase(full + sk, phase, &abort_flag)) failed();
+    const int base = un.p * KV8_PAGE, key0 = base + 16 * (g >> 1) + (g & 1);
+    const bool whole = base + KV8_PAGE <= least_seen;            // every row sees every key
+    float s[4][4];
+    if (live) {
+      // the four steps' sums are independent: their products go round, so that none waits for its own last one
+      const uint4* row = reinterpret_cast<const uint4*>(ring + sk * S::SLOT + (16 * (g >> 1) + (g & 1)) * 64 + c * 16);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[y][x] = 0.f;
+#pragma unroll
+      for (int h = 0; h < DH / 64; ++h) {
+        uint4 k0[4], k1[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          k0[y] = row[y * 16 + h * 256];
+          k1[y] = row[y * 16 + h * 256 + 8];
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            uint32_t fa[4];
+            kv8_half4<KIND>(reinterpret_cast<const uint32_t*>(&k0[y])[x], fa[0], fa[2]);
+            kv8_half4<KIND>(reinterpret_cast<const uint32_t*>(&k1[y])[x], fa[1], fa[3]);
+            mma_f16(s[y], fa, qf[h][x][0], qf[h][x][1]);
+          }
+      }
+    }
+    uint32_t pf[4][2];
+    float keep[2], scale_v[2];
+    if (live) {
+      if (!whole) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (key0 + 4 * y + 2 * (x >> 1) >= seen[x & 1]) s[y][x] = -INFINITY;
+      }
+      float sub[2], fk[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = max3(fmaxf(s[0][i], s[0][2 + i]), fmaxf(s[1][i], s[1][2 + i]), max3(s[2][i], s[2][2 + i], fmaxf(s[3][i], s[3][2 + i])));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        fk[i] = f[i] * ks;
+        const float mn = fmaxf(m[i], mx * fk[i]);
+        const float base_m = mn == -INFINITY ? 0.f : mn;
+        keep[i] = fast_exp2(m[i] - base_m);
+        m[i] = mn;
+        sub[i] = KA_SHIFT - base_m;
+        scale_v[i] = base < seen[i] ? vs : 0.f;                  // a row that sees none of it takes none, NaN neither
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[y][x] = fast_exp2(fmaf(s[y][x], fk[x & 1], sub[x & 1]));
+      if (!whole) {                                              // whatever the scale of the keys is
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (key0 + 4 * y + 2 * (x >> 1) >= seen[x & 1]) s[y][x] = 0.f;
+      }
+      // the columns' sums of the rounded weights: a product with ones
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        pf[y][0] = transpose8(half2_bits(s[y][0], s[y][1]));
+        pf[y][1] = transpose8(half2_bits(s[y][2], s[y][3]));
+        mma_f16(sum, ones, pf[y][0], pf[y][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) l[i] = fmaf(l[i], keep[i], sum[i]);
+    }
+    if (live && !dead && !wait_phase(full + sv, phase, &abort_flag)) failed();
+    if (live) {
+      if (!whole) {
+        // codes of values behind what any row sees may be anything (not a number even): zero times them is not zero
+        const int left = all_seen - base;
+#pragma unroll 1
+        for (int i = lane; i < DH * 16; i += 32) {
+          const int over = left - (i & 15) * 4;                  // word i & 15 of a row has four tokens
+          if (over < 4) reinterpret_cast<uint32_t*>(ring + sv * S::SLOT)[i] &= over <= 0 ? 0u : (1u << (8 * over)) - 1u;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {       // a maximum has grown (or is NaN)
+#pragma unroll
+        for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[d][x] *= keep[x & 1];
+      }
+      const unsigned char* vb = ring + sv * S::SLOT + g * 64 + c * 16;
+      // four rows of results at a time, for the same reason
+#pragma unroll
+      for (int d0 = 0; d0 < DH / 16; d0 += 4) {
+        uint4 v0[4], v1[4];
+        float op[4][4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          v0[d] = *reinterpret_cast<const uint4*>(vb + (d0 + d) * 1024);
+          v1[d] = *reinterpret_cast<const uint4*>(vb + (d0 + d) * 1024 + 512);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) op[d][x] = 0.f;
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            uint32_t fa[4];
+            kv8_half4<KIND>(reinterpret_cast<const uint32_t*>(&v0[d])[y], fa[0], fa[2]);
+            kv8_half4<KIND>(reinterpret_cast<const uint32_t*>(&v1[d])[y], fa[1], fa[3]);
+            mma_f16(op[d], fa, pf[y][0], pf[y][1]);
+          }
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[d0 + d][x] = fmaf(op[d][x], scale_v[x & 1], o[d0 + d][x]);
+      }
+    }
+    __syncwarp();
+    done += live;
+    if (un.flags & UNIT_LAST) {
+      // ---- the tile's last page here: its result, or its part of it
+      const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (un.flags & UNIT_FIRST ? 0 : 1);
+#pragma unroll
+      for (int i2 = 0; i2 < 2; ++i2) {
+        const int r = 2 * c + i2, rr = un.tile * QR + r;
+        if (rr >= total) continue;
+        if (un.flags & UNIT_WHOLE) {
+          const float inv = ctx - rows + rr / a.group + 1 > 0 ? 1.f / l[i2] : 0.f;
+          __nv_bfloat16* dst = a.out + static_cast<size_t>(first + rr / a.group) * a.ldo + (un.head * a.group + rr % a.group) * DH + g;
+#pragma unroll
+          for (int d = 0; d < DH / 16; ++d) {
+            dst[d * 16] = __float2bfloat16(o[d][i2] * inv);
+            dst[d * 16 + 8] = __float2bfloat16(o[d][2 + i2] * inv);
+          }
+        } else {
+          float* dst = a.part_o + (slot * QR + r) * DH + g;
+#pragma unroll
+          for (int d = 0; d < DH / 16; ++d) {
+            dst[d * 16] = o[d][i2];
+            dst[d * 16 + 8] = o[d][2 + i2];
+          }
+          if (g == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * QR + r) * 2) = make_float2(m[i2], l[i2]);
+        }
+      }
+    }
+    }
+    if (i + AHEAD < n_units) ask(i + AHEAD);
+  }
+}
+
+// Tiles that lie in more than one CTA: the CTA behind the tile's first boundary has its block here.  The warps take the
+// parts in turn.
+constexpr int KM_WARPS = 16;
+template <int DH>
+__global__ void __launch_bounds__(32 * KM_WARPS) kv8_attn_merge_kernel(const __grid_constant__ Kv8Attn a) {
+  constexpr int QR = KA_ROWS, PER = DH / 32;
+  __shared__ float s_max[KM_WARPS], s_sum[KM_WARPS];
+  __shared__ float s_o[KM_WARPS][DH];
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // the parts are complete
+  const int b = blockIdx.x + 1;
+  const Kv8Desc d = a.desc[b];
+  const long long at = static_cast<long long>(d.share) * b;
+  // starts here, ends before, or has begun before the last boundary
+  if (at >= d.units || d.lo >= at || d.hi <= at || d.lo < at - d.share) return;
+  const int parts = static_cast<int>((d.hi - at + d.share - 1) / d.share) + 1;
+  const size_t s0 = static_cast<size_t>(b - 1) * 2 + (d.lo == at - d.share ? 0 : 1);
+  auto slot = [&](int i) { return i == 0 ? s0 : static_cast<size_t>(b - 1 + i) * 2; };
+  const Kv8Entry x = kv8_entry(a, d.entry);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_rows = min(QR, x.rows * a.group - d.tile * QR);
+  const int ctx = min(x.ctx, a.c.max_pages * KV8_PAGE);
+  // warp w has row w mod n_rows, and of its parts every subs-th from w / n_rows on
+  const int r = warp % n_rows, sub = warp / n_rows, subs = KM_WARPS / n_rows;
+  const int mine = sub < subs && sub < parts ? (parts - sub + subs - 1) / subs : 0;
+  auto ml = [&](int i) { return *reinterpret_cast<const float2*>(a.part_ml + (slot(sub + subs * i) * QR + r) * 2); };
+  float gm = -INFINITY, gl = 0.f, o[PER];
+  for (int i = lane; i < mine; i += 32) gm = fmaxf(gm, ml(i).x);
+  gm = warp_max(gm);
+  if (lane == 0) s_max[warp] = gm;
+#pragma unroll
+  for (int y = 0; y < PER; ++y) o[y] = 0.f;
+  __syncthreads();
+  for (int w = r; w < subs * n_rows; w += n_rows) gm = fmaxf(gm, s_max[w]);
+  for (int i0 = 0; i0 < mine; i0 += 32) {
+    float k = 0.f;
+    if (i0 + lane < mine) {
+      const float2 v = ml(i0 + lane);
+      k = part_weight(v.x, v.y, gm);
+      if (k != 0.f) gl += k * v.y;
+    }
+    const int n = min(32, mine - i0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float ki = __shfl_sync(0xffffffffu, k, i);
+      const float* src = a.part_o + (slot(sub + subs * (i0 + i)) * QR + r) * DH + lane * PER;
+#pragma unroll
+      for (int y = 0; y < PER; ++y) o[y] = fmaf(ki, src[y], o[y]);
+    }
+  }
+  gl = warp_sum(gl);
+  if (lane == 0) s_sum[warp] = gl;
+#pragma unroll
+  for (int y = 0; y < PER; ++y) s_o[warp][lane * PER + y] = o[y];
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_rows * DH; e += 32 * KM_WARPS) {
+    const int er = e / DH, ch = e % DH, rr = d.tile * QR + er;
+    float v = 0.f, sum = 0.f;
+    for (int w = er; w < subs * n_rows; w += n_rows) {
+      v += s_o[w][ch];
+      sum += s_sum[w];
+    }
+    const bool any = ctx - x.rows + rr / a.group + 1 > 0;
+    a.out[static_cast<size_t>(x.first + rr / a.group) * a.ldo + (d.head * a.group + rr % a.group) * DH + ch] =
+        __float2bfloat16(any ? v / sum : 0.f);
+  }
+}
+
+template <int KIND, int DH>
+static int launch_attn(const Kv8Attn& a, int ctas, cudaStream_t st) {
+  using S = Kv8Smem<DH>;
+  static bool set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -4;
+  if (dev >= 64 || !set[dev]) {
+    if (cudaFuncSetAttribute(kv8_attn_kernel<KIND, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES) != cudaSuccess)
+      return -4;
+    if (dev < 64) set[dev] = true;
+  }
+  kv8_attn_kernel<KIND, DH><<<ctas, 32, S::BYTES, st>>>(a);
+  if (ctas > 1) {
+    // launched while the first kernel runs; it waits for that one's end itself
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = ctas - 1;
+    cfg.blockDim = 32 * KM_WARPS;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kv8_attn_merge_kernel<DH>, a) != cudaSuccess) return -3;
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace cb
 
 using namespace cb;
 
+// Units of an entry at most; entries of a launch; CTAs of a launch: one for every place on the device, where there is work.
+static long long attn_units(int most, int group, int max_pages, int kv_heads) {
+  return (1ll * most * group + KA_ROWS - 1) / KA_ROWS * (max_pages + KA_EXTRA) * kv_heads;
+}
+static int attn_entries(int n, long long units) {
+  const long long fit = 0x7fffffffll / units;
+  return static_cast<int>(fit < n && fit < KA_ENTRIES ? fit : n < KA_ENTRIES ? n : KA_ENTRIES);
+}
+static int attn_ctas(int n, long long units, int dh) {
+  const long long places = static_cast<long long>(dh == 64 ? KA_PLACES64 : KA_PLACES) * sm_count(), work = (n * units + KA_SHARE - 1) / KA_SHARE;
+  return static_cast<int>(work < places ? work : places);
+}
+
+// Bytes of scratch of one call.
+extern "C" int64_t cb_kv8_attn_scratch(int n, int rows, int most, int group, int max_pages, int kv_heads, int dh) {
+  const long long units = attn_units(most < rows ? most : rows, group, max_pages, kv_heads);
+  return attn_ctas(n < KA_ENTRIES ? n : KA_ENTRIES, units, dh) * static_cast<int64_t>(2 * KA_ROWS * (dh + 2) * 4 + sizeof(Kv8Desc)) + 256;
+}
+
 extern "C" int cb_kv8_attn(const void* q, int ldq, const void* k_cache, const void* v_cache, const float* k_scale,
                            const float* v_scale, const int* page_table, int max_pages, int num_pages, int kv_heads,
                            int dh, int kind, const int* ctx, const int* row0, int n, int rows, int most, int heads,
-                           float scale, void* out, int ldo, int* status, void* stream) {
+                           float scale, void* out, int ldo, void* scratch, int* status, void* stream) {
   if (n < 1 || rows < 1 || most < 1 || kv_heads < 1 || heads < 1 || heads % kv_heads != 0) return -1;
   if ((dh != 64 && dh != 128) || (kind != KV8_INT8 && kind != KV8_E4M3)) return -2;
+  const int group = heads / kv_heads;
+  if (most > rows) most = rows;                                // a row counts at most once
+  const long long units = attn_units(most, group, max_pages, kv_heads);
+  if (1ll * max_pages * KV8_PAGE > 0x7fffffffll || units > 0x7fffffffll) return -5;
+  const int each = attn_entries(n, units), ctas = attn_ctas(each, units, dh);
   Kv8Attn a;
-  a.c = Kv8Cache{static_cast<uint8_t*>(const_cast<void*>(k_cache)), static_cast<uint8_t*>(const_cast<void*>(v_cache)),
-                 const_cast<float*>(k_scale), const_cast<float*>(v_scale), page_table, max_pages, num_pages, kv_heads};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
-  a.ldq = ldq; a.ldo = ldo; a.heads = heads; a.ctx = ctx; a.row0 = row0; a.rows = rows; a.most = most;
+  a.ldq = ldq; a.ldo = ldo; a.group = group; a.rows = rows; a.most = most;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.desc = static_cast<Kv8Desc*>(scratch);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(Kv8Desc) + 255) / 256 * 256);
+  a.part_ml = a.part_o + static_cast<size_t>(ctas) * 2 * KA_ROWS * dh;
   a.status = status;
-  const long long blocks = 1ll * n * most * heads;
-  if (blocks > 0x7fffffffll) return -4;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CB_ATTN(KIND_, DH_) \
-  kv8_attn_kernel<KIND_, DH_><<<static_cast<unsigned>(blocks), KA_WARPS * 32, 0, st>>>(a)
-  if (kind == KV8_INT8) {
-    if (dh == 64) CB_ATTN(KV8_INT8, 64); else CB_ATTN(KV8_INT8, 128);
-  } else {
-    if (dh == 64) CB_ATTN(KV8_E4M3, 64); else CB_ATTN(KV8_E4M3, 128);
+  for (int e0 = 0; e0 < n; e0 += each) {
+    a.c = Kv8Cache{static_cast<uint8_t*>(const_cast<void*>(k_cache)), static_cast<uint8_t*>(const_cast<void*>(v_cache)),
+                   const_cast<float*>(k_scale), const_cast<float*>(v_scale),
+                   page_table + static_cast<size_t>(e0) * max_pages, max_pages, num_pages, kv_heads};
+    a.ctx = ctx + e0;
+    a.row0 = row0 != nullptr ? row0 + e0 : nullptr;
+    a.first = e0;
+    a.n = n - e0 < each ? n - e0 : each;
+    int rc;
+    if (kind == KV8_INT8) rc = dh == 64 ? launch_attn<KV8_INT8, 64>(a, ctas, st) : launch_attn<KV8_INT8, 128>(a, ctas, st);
+    else rc = dh == 64 ? launch_attn<KV8_E4M3, 64>(a, ctas, st) : launch_attn<KV8_E4M3, 128>(a, ctas, st);
+    if (rc != 0) return rc;
   }
-#undef CB_ATTN
-  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+  return 0;
 }

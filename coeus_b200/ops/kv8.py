@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -74,6 +75,8 @@ def _check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, ints, row0
             continue
         if not t.is_contiguous():
             raise ValueError(f"{what}: cache, tables and lengths have to be contiguous")
+        if t.is_cuda and t.data_ptr() % 16 and t.dim() > 2:
+            raise ValueError(f"{what}: the cache has to start at a multiple of 16 bytes")
         if t.device != k_cache.device:
             raise ValueError(f"{what}: tensors on {t.device} and {k_cache.device}")
     return pages, heads, dh
@@ -242,6 +245,13 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
     return out[0], out[1]
 
 
+@lru_cache(maxsize=1024)
+def _scratch(*shape: int) -> int:
+    fn = _lib.lib().cb_kv8_attn_scratch
+    fn.restype = ctypes.c_int64
+    return fn(*shape)
+
+
 def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
                   ctx_len: torch.Tensor, nh: int, row0: Optional[torch.Tensor] = None,
@@ -259,6 +269,8 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if row0 is None and n > rows:
         raise ValueError(f"kv8_attention: {n} entries, {rows} rows")
     scale = scale if scale is not None else 1.0 / math.sqrt(dh)
+    if not 0.0 <= scale < math.inf:
+        raise ValueError(f"kv8_attention: scale {scale}")
     if q.is_cuda:
         whole = row0 is None and n == rows           # every row is written
         out = (torch.empty if whole else torch.zeros)((rows, nh * dh), dtype=torch.bfloat16,
@@ -266,13 +278,16 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         if n == 0 or rows == 0:
             return out
         with torch.cuda.device(q.device):
+            scratch = torch.empty(_scratch(n, rows, max_rows, nh // heads,
+                                           page_table.shape[1], heads, dh), dtype=torch.uint8,
+                                  device=q.device)
             rc = _lib.lib().cb_kv8_attn(
                 _lib.ptr(q), q.stride(0), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale),
                 _lib.ptr(v_scale), _lib.ptr(page_table), page_table.shape[1], pages, heads, dh,
                 int(k_cache.dtype != torch.int8), _lib.ptr(ctx_len), _lib.ptr(row0), n, rows,
                 max_rows, nh, ctypes.c_float(scale), _lib.ptr(out), out.stride(0),
-                _lib.ptr(_lib.status_buffer(q.device)), _lib.stream_ptr())
-        _lib.check_rc(rc, "cb_kv8_attn")
+                _lib.ptr(scratch), _lib.ptr(_lib.status_buffer(q.device)), _lib.stream_ptr())
+        _lib.check_rc(rc, "cb_kv8_attn", launches=2 * ((n + 255) // 256))
         return out
     out = torch.zeros((rows, nh * dh), dtype=q.dtype)
     g = nh // heads

@@ -111,6 +111,41 @@ def test_attention_long_context(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,dh,group,rows", [(6, 128, 3, 1), (6, 64, 1, 1), (3, 128, 3, 5), (4, 64, 4, 4)])
+def test_attention_many_pages_per_block(kind, heads, dh, group, rows):
+    """Enough pages that the ring of every block goes round several times, over several tiles."""
+    n = 70
+    lens = [1 + (i * 997) % 6000 for i in range(n)]
+    c = Case(kind, heads, dh, lens, DEV)
+    k = torch.randn(max(lens), heads * dh, generator=c.gen).bfloat16().to(DEV)
+    v = torch.randn(max(lens), heads * dh, generator=c.gen).bfloat16().to(DEV)
+    table = c.table.to(DEV)
+    for e in range(n):
+        kv8.kv8_write(k[:lens[e]], v[:lens[e]], *c.c, table[e:e + 1], i32([0], DEV),
+                      row0=i32([0, lens[e]], DEV), max_rows=lens[e])
+    counts = [1 if rows == 1 else min(1 + e % rows, lens[e]) for e in range(n)]
+    q = torch.randn(sum(counts), heads * group * dh, generator=c.gen).bfloat16()
+    got = c.attend(q, lens, counts, heads * group).double()
+    # what the cache holds of the longest entry's first page differs from entry to entry only by
+    # the scale of their last pages: read it back and compare in 64 bits
+    at = 0
+    for e in range(n):
+        kk, vv = kv8.kv8_read(*c.c, table[e:e + 1], i32([0], DEV), i32([0, lens[e]], DEV), lens[e], lens[e])
+        kk = kk.double().view(lens[e], heads, dh).transpose(0, 1)
+        vv = vv.double().view(lens[e], heads, dh).transpose(0, 1)
+        x = q[at:at + counts[e]].to(DEV).double().view(counts[e], heads, group, dh).permute(1, 2, 0, 3)
+        s = torch.einsum("hgrd,hcd->hgrc", x, kk) * dh ** -0.5
+        seen = torch.arange(lens[e], device=DEV)[None] <= (lens[e] - counts[e] + torch.arange(counts[e], device=DEV))[:, None]
+        w = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        want = torch.einsum("hgrc,hcd->rhgd", w, vv).reshape(counts[e], -1)
+        spread = torch.einsum("hgrc,hcd->rhgd", w, vv.abs()).reshape(counts[e], -1)
+        err = (got[at:at + counts[e]] - want).abs()
+        assert (err <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * spread + 1e-30).all(), e
+        at += counts[e]
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_scales_apart(kind):
     """Pages whose values differ by 2^30, and a row that only listens to the small ones."""
     c = Case(kind, 1, 64, [192], DEV)

@@ -19,31 +19,63 @@
 namespace cb {
 
 constexpr int BEAM_MAX = 32;           // beams of a request
-constexpr int BLK = 1024;              // logits of a block
-constexpr int PICK_THREADS = 256;
+constexpr int BLK = 512;               // logits of a block (ops/beam.py sizes the scratch by it)
+constexpr int PICK_THREADS = 512;
+constexpr int PICK_PER = 6;            // blocks that a thread keeps the values of
 constexpr int PICK_CAP = 1024;         // continuations compared at once
 
+// Blocks begin at multiples of 16 bytes, so that a row that does not is read in vectors all the same: block k of a row
+// whose first logit is `skew` logits behind such a place has logits k BLK - skew .. (k + 1) BLK - skew - 1, as far as
+// there are any.
 template <typename T>
-__device__ __forceinline__ float beam_logit(const T* p) {
-  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
-  else return *p;
+__device__ __forceinline__ int beam_skew(const T* row) {
+  return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16) / static_cast<int>(sizeof(T));
+}
+__device__ __forceinline__ float beam_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float beam_logit(const float* p) { return *p; }
+// 16 bytes of logits; `lo` and `hi` cut off what is not the row's.
+template <typename T>
+__device__ __forceinline__ void beam_vector(const T* row, int t, int V, float* x) {
+  constexpr int N = 16 / sizeof(T);
+  if (t >= 0 && t + N <= V) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + t));
+    if constexpr (N == 8) {
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 b = unpack_bf16x2(v[i]);
+        x[2 * i] = b.x;
+        x[2 * i + 1] = b.y;
+      }
+    } else {
+      x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = t + i >= 0 && t + i < V ? beam_logit(row + t + i) : -INFINITY;
+  }
 }
 
+constexpr int PASS_WARPS = 4;
 template <typename T>
-__global__ void __launch_bounds__(256) beam_pass_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk,
-                                                        const float* __restrict__ scores,
-                                                        const uint8_t* __restrict__ done, float2* __restrict__ part) {
-  const int row = blockIdx.y, blk = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(32 * PASS_WARPS) beam_pass_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk,
+                                                                    const float* __restrict__ scores,
+                                                                    const uint8_t* __restrict__ done, float2* __restrict__ part) {
+  constexpr int N = 16 / sizeof(T), PER = BLK / 32;              // logits of a vector, of a lane
+  const int row = blockIdx.y, blk = blockIdx.x * PASS_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (blk >= nblk || done[row] || scores[row] == -INFINITY) return;
   const T* x = logits + row * ld;
-  const int t0 = blk * BLK, t1 = min(V, t0 + BLK);
-  float m = -INFINITY, s = 0.f;
-  for (int t = t0 + lane; t < t1; t += 32) m = fmaxf(m, beam_logit(x + t));
+  const int t0 = blk * BLK - beam_skew(x) + lane * N;
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < PER / N; ++i) beam_vector(x, t0 + i * 32 * N, V, v + i * N);
+  float m = v[0], s = 0.f;
+#pragma unroll
+  for (int i = 1; i < PER; ++i) m = fmaxf(m, v[i]);
   m = warp_max(m);
-  for (int t = t0 + lane; t < t1; t += 32) {
-    const float v = beam_logit(x + t);
-    s += v == -INFINITY ? 0.f : expf(v - m);             // NaN and +inf make the sum NaN
-  }
+  const float base = m == -INFINITY ? 0.f : m;                   // nothing but -inf: the sum is 0
+#pragma unroll
+  for (int i = 0; i < PER; ++i) s += expf(v[i] - base);          // NaN and +inf make it NaN
   s = warp_sum(s);
   if (lane == 0) part[static_cast<size_t>(row) * nblk + blk] = make_float2(m, s);
 }
@@ -88,13 +120,15 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
     const float2* p = part + static_cast<size_t>(row0 + j) * nblk;
     double lse = NEG;
     if (!done[row0 + j] && scores[row0 + j] != -INFINITY) {
+      // in fp64 but for the factors of the blocks: their errors (2 units of fp32 each) average out like those of the
+      // logits' own exponentials
       float m = -INFINITY;
       for (int i = lane; i < nblk; i += 32) m = fmaxf(m, p[i].x);
       m = warp_max(m);
       double s = 0.0;
       for (int i = lane; i < nblk; i += 32) {
         const float2 q = p[i];
-        s += q.x == -INFINITY && q.y == 0.f ? 0.0 : static_cast<double>(q.y) * exp(static_cast<double>(q.x) - static_cast<double>(m));
+        s += q.x == -INFINITY && q.y == 0.f ? 0.0 : static_cast<double>(q.y) * static_cast<double>(expf(q.x - m));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -110,21 +144,33 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
     return v == v ? v : NEG;
   };
   // the K best blocks, one after the other; an ended beam is one block
+  auto block_value = [&](int i) {
+    const int j = i / nblk, k = i % nblk;
+    double v = NEG;
+    if (done[row0 + j]) {
+      if (k == 0 && eos >= 0) v = scores[row0 + j];
+      if (v != v) v = NEG;
+    } else if (scores[row0 + j] != -INFINITY) {
+      v = value(j, part[static_cast<size_t>(row0 + j) * nblk + k].x);
+    }
+    return v;
+  };
   int found = 0;
   Best last{INFINITY, -1};
+  double mine[PICK_PER];                                         // a thread keeps its first ones
+#pragma unroll
+  for (int u = 0; u < PICK_PER; ++u) {
+    const int i = threadIdx.x + u * PICK_THREADS;
+    mine[u] = i < K * nblk ? block_value(i) : NEG;
+  }
   for (; found < K; ++found) {
     Best b{NEG, 0x7fffffffffffffffll};
-    for (int i = threadIdx.x; i < K * nblk; i += PICK_THREADS) {
-      const int j = i / nblk, k = i % nblk;
-      double v = NEG;
-      if (done[row0 + j]) {
-        if (k == 0 && eos >= 0) v = scores[row0 + j];
-        if (v != v) v = NEG;
-      } else if (scores[row0 + j] != -INFINITY) {
-        v = value(j, part[static_cast<size_t>(row0 + j) * nblk + k].x);
-      }
+    auto look = [&](double v, int i) {
       if (v > NEG && better(v, i, b) && !better(v, i, last) && i != last.at) b = Best{v, i};
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < PICK_PER; ++u) look(mine[u], threadIdx.x + u * PICK_THREADS);
+    for (int i = threadIdx.x + PICK_PER * PICK_THREADS; i < K * nblk; i += PICK_THREADS) look(block_value(i), i);
     b = block_best(b, red);
     if (!(b.v > NEG)) break;
     if (threadIdx.x == 0) s_blk[found] = b.at;
@@ -141,8 +187,8 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
         continue;
       }
       const T* x = logits + (row0 + j) * ld;
-      const int t1 = min(V, (k + 1) * BLK);
-      for (int t = k * BLK + threadIdx.x; t < t1; t += PICK_THREADS) f(value(j, beam_logit(x + t)), static_cast<int64_t>(j) * V + t);
+      const int t0 = k * BLK - beam_skew(x);
+      for (int t = max(0, t0) + threadIdx.x; t < min(V, t0 + BLK); t += PICK_THREADS) f(value(j, beam_logit(x + t)), static_cast<int64_t>(j) * V + t);
     }
   };
   each([&](double v, int64_t at) {
@@ -296,7 +342,16 @@ __global__ void __launch_bounds__(256) beam_copy_kernel(const __grid_constant__ 
   char* to = static_cast<char*>(a.base[blockIdx.y]) + d * bytes;
   const size_t first = blockIdx.z * static_cast<size_t>(blockDim.x) + threadIdx.x, step = gridDim.z * static_cast<size_t>(blockDim.x);
   if (((reinterpret_cast<uintptr_t>(a.base[blockIdx.y]) | bytes) & 15) == 0) {
-    for (size_t i = first; i < bytes / 16; i += step) reinterpret_cast<uint4*>(to)[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+    const size_t n = bytes / 16;
+    size_t i = first;
+    for (; i + 3 * step < n; i += 4 * step) {            // four loads on their way
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = __ldg(reinterpret_cast<const uint4*>(from) + i + u * step);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) reinterpret_cast<uint4*>(to)[i + u * step] = v[u];
+    }
+    for (; i < n; i += step) reinterpret_cast<uint4*>(to)[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
   } else {
     for (size_t i = first; i < bytes / 4; i += step) reinterpret_cast<uint32_t*>(to)[i] = __ldg(reinterpret_cast<const uint32_t*>(from) + i);
   }
@@ -306,23 +361,21 @@ __global__ void __launch_bounds__(256) beam_copy_kernel(const __grid_constant__ 
 
 using namespace cb;
 
-extern "C" int cb_beam_block() { return BLK; }
-
-// part: float2 [B K, ceil(V / cb_beam_block())] scratch
+// part: float2 [B K, ceil((V + 7) / BLK)] scratch
 extern "C" int cb_beam_select(const void* logits, int64_t ld, int f32, int B, int K, int V, const float* scores,
                               const void* done, int eos, void* part, float* out_score, int64_t* out_parent,
                               int64_t* out_token, void* out_done, void* stream) {
   if (B < 1 || K < 1 || K > BEAM_MAX || V < 1 || eos >= V) return -1;
-  const int nblk = (V + BLK - 1) / BLK;
+  const int nblk = (V + 7 + BLK - 1) / BLK;                       // a row may begin up to seven logits into its first block
   if (1ll * B * K > 65535) return -2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((nblk + 7) / 8, B * K);
+  const dim3 grid((nblk + PASS_WARPS - 1) / PASS_WARPS, B * K);
   auto* P = static_cast<float2*>(part);
   auto* D = static_cast<const uint8_t*>(done);
   auto* OD = static_cast<uint8_t*>(out_done);
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    beam_pass_kernel<T><<<grid, 256, 0, st>>>(x, ld, V, nblk, scores, D, P);
+    beam_pass_kernel<T><<<grid, 32 * PASS_WARPS, 0, st>>>(x, ld, V, nblk, scores, D, P);
     beam_pick_kernel<T><<<B, PICK_THREADS, 0, st>>>(x, ld, V, nblk, K, scores, D, eos, P, out_score, out_parent, out_token, OD);
   };
   if (f32) go(static_cast<const float*>(logits));

@@ -27,19 +27,6 @@ struct Kv8Cache {
   int max_pages, num_pages, heads;
 };
 
-template <int KIND>
-__device__ __forceinline__ float kv8_value(uint8_t c) {
-  if constexpr (KIND == KV8_INT8) return static_cast<float>(static_cast<int8_t>(c));
-  else return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-}
-// Nearest code of x (ties to even); |x| is at most the largest code, or x is not finite and the
-// block's scale is NaN: such a code is 0.
-template <int KIND>
-__device__ __forceinline__ uint8_t kv8_code(float x) {
-  if (!(fabsf(x) <= 448.f)) x = 0.f;
-  if constexpr (KIND == KV8_INT8) return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(x)));
-  else return static_cast<uint8_t>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
-}
 // Smallest e >= -126 with amax <= largest code * 2^e, from the bits of a finite fp32 amax.
 template <int KIND>
 __device__ __forceinline__ int kv8_exponent(float amax) {

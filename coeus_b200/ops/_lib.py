@@ -129,6 +129,50 @@ def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+class _SameDevice:
+    """``with`` over nothing: the device is the current one already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_same_device = _SameDevice()
+
+
+def on_device(index: int):
+    """Makes CUDA device ``index`` the current one for a launch (nothing to do, and nothing paid, if it
+    is)."""
+    if _raw_device is not None and _raw_device() == index:
+        return _same_device
+    return torch.cuda.device(index)
+
+
+_signed: set = set()
+
+
+def entry(name: str, signature: str):
+    """The library's entry point ``name`` with its argument types set (``p`` pointer, ``i`` int, ``l``
+    int64, ``f`` float), so that a call takes plain numbers: an object per pointer was a third of the host time
+    of a small operator."""
+    fn = getattr(lib(), name)
+    if name not in _signed:
+        plain = getattr(_lib, name)
+        plain.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64,
+                           "f": ctypes.c_float}[c] for c in signature]
+        _signed.add(name)
+    return fn
+
+
+def stream_int() -> int:
+    """The current stream of the current device as a number."""
+    if _raw_stream is not None and _raw_device is not None:
+        return _raw_stream(_raw_device())
+    return torch.cuda.current_stream().cuda_stream
+
+
 _status_bufs: dict = {}
 
 

@@ -12,6 +12,7 @@ from . import _lib
 from .decode import PAGE
 
 MAX_BEAMS = 32
+BLOCK = 512            # logits that the kernels sum up at a time (csrc/beam.cu)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor,
@@ -40,10 +41,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor,
     V = logits.shape[1]
     if eos_id is not None and not 0 <= eos_id < V:
         raise ValueError(f"beam_select: eos_id {eos_id} is outside the vocabulary of {V}")
-    if not (logits.device == scores.device == done.device):
+    device = logits.get_device()
+    if scores.get_device() != device or done.get_device() != device:
         raise ValueError("beam_select: tensors on different devices")
-    if logits.is_cuda:
-        if logits.dtype not in (torch.bfloat16, torch.float32):
+    if device >= 0:
+        f32 = logits.dtype == torch.float32
+        if not f32 and logits.dtype != torch.bfloat16:
             raise ValueError(f"beam_select: logits in bf16 or fp32, not {logits.dtype}")
         if V > 1 << 26 or B * K > 65535:
             raise ValueError(f"beam_select: {B * K} rows of {V} logits are too many")
@@ -51,19 +54,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor,
             logits = logits.contiguous()
         scores, done = scores.contiguous(), done.contiguous()
         dev = logits.device
-        lib = _lib.lib()
-        blocks = (V + lib.cb_beam_block() - 1) // lib.cb_beam_block()
-        part = torch.empty((B * K, blocks, 2), dtype=torch.float32, device=dev)
-        out = torch.empty((B, K), dtype=torch.float32, device=dev)
-        parent = torch.empty((B, K), dtype=torch.int64, device=dev)
-        token, ended = torch.empty_like(parent), torch.empty_like(done)
+        part = torch.empty(B * K * ((V + 7 + BLOCK - 1) // BLOCK) * 2, dtype=torch.float32, device=dev)
+        out, parent = torch.empty_like(scores), torch.empty((2, B, K), dtype=torch.int64, device=dev)
+        parent, token = parent.unbind(0)
+        ended = torch.empty_like(done)
         if B:
-            with torch.cuda.device(dev):
-                rc = lib.cb_beam_select(
-                    _lib.ptr(logits), ctypes.c_int64(logits.stride(0)),
-                    int(logits.dtype == torch.float32), B, K, V, _lib.ptr(scores), _lib.ptr(done),
-                    -1 if eos_id is None else eos_id, _lib.ptr(part), _lib.ptr(out),
-                    _lib.ptr(parent), _lib.ptr(token), _lib.ptr(ended), _lib.stream_ptr())
+            with _lib.on_device(device):
+                rc = _lib.entry("cb_beam_select", "pliiiippipppppp")(
+                    logits.data_ptr(), logits.stride(0), int(f32), B, K, V, scores.data_ptr(),
+                    done.data_ptr(), -1 if eos_id is None else eos_id, part.data_ptr(),
+                    out.data_ptr(), parent.data_ptr(), token.data_ptr(), ended.data_ptr(),
+                    _lib.stream_int())
             _lib.check_rc(rc, "cb_beam_select", launches=2)
         return out, parent, token, ended
     x = logits.double().view(B, K, V)
@@ -112,7 +113,9 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
         raise ValueError(f"beam_pages: length is int32 [{B}]")
     if pool.dim() != 2 or pool.shape[0] != B or pool.dtype != torch.int32:
         raise ValueError(f"beam_pages: the pool is int32 [{B}, pages]")
-    if not (page_table.device == parent.device == length.device == pool.device):
+    device = page_table.get_device()
+    if parent.get_device() != device or length.get_device() != device \
+            or pool.get_device() != device:
         raise ValueError("beam_pages: tensors on different devices")
     if not 1 <= num_pages <= 200 * 1024 * 8:
         raise ValueError(f"beam_pages: a cache of 1 to {200 * 1024 * 8} pages, not {num_pages}")
@@ -120,15 +123,15 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
     page_table, parent, length, pool = (t.contiguous() for t in (page_table, parent, length, pool))
     table = torch.empty_like(page_table)
     moves = torch.empty((2, B * K), dtype=torch.int32, device=dev)
-    src, dst = moves[0], moves[1]
+    src, dst = moves.unbind(0)
     if B == 0:
         return table, src, dst
-    if page_table.is_cuda:
-        with torch.cuda.device(dev):
-            rc = _lib.lib().cb_beam_pages(
-                _lib.ptr(page_table), width, B, K, _lib.ptr(parent), _lib.ptr(length),
-                _lib.ptr(pool), pool.shape[1], num_pages, _lib.ptr(table), _lib.ptr(src),
-                _lib.ptr(dst), _lib.ptr(_lib.status_buffer(dev)), _lib.stream_ptr())
+    if device >= 0:
+        with _lib.on_device(device):
+            rc = _lib.entry("cb_beam_pages", "piiipppiippppp")(
+                page_table.data_ptr(), width, B, K, parent.data_ptr(), length.data_ptr(),
+                pool.data_ptr(), pool.shape[1], num_pages, table.data_ptr(), src.data_ptr(),
+                dst.data_ptr(), _lib.status_buffer(dev).data_ptr(), _lib.stream_int())
         _lib.check_rc(rc, "cb_beam_pages")
         return table, src, dst
     moves.fill_(-1)
@@ -167,22 +170,28 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
         raise ValueError("copy_pages: src and dst are int32 of one length")
     if not caches or src.numel() == 0:
         return
-    pages = caches[0].shape[0]
+    pages, device, n = caches[0].shape[0], src.get_device(), len(caches)
+    if dst.get_device() != device:
+        raise ValueError("copy_pages: tensors on different devices")
+    base, sizes, odd = [], [], 0
     for c in caches:
         if not c.is_contiguous() or c.dim() < 1 or c.shape[0] != pages:
             raise ValueError("copy_pages: contiguous tensors with one number of pages")
-        if not (c.device == src.device == dst.device):
+        if c.get_device() != device:
             raise ValueError("copy_pages: tensors on different devices")
-    if caches[0].is_cuda:
-        sizes = [c[0].numel() * c.element_size() for c in caches]
-        if any(s < 4 or s % 4 for s in sizes) or any(c.data_ptr() % 4 for c in caches):
+        base.append(c.data_ptr())
+        sizes.append(c.numel() // max(1, pages) * c.element_size())
+        odd |= base[-1] | sizes[-1]
+    if device >= 0:
+        if odd % 4 or 0 in sizes:
             raise ValueError("copy_pages: a page is a multiple of four bytes")
-        n = len(caches)
-        with torch.cuda.device(src.device):
-            rc = _lib.lib().cb_beam_copy(
-                (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches]), (ctypes.c_int * n)(*sizes),
-                n, _lib.ptr(src.contiguous()), _lib.ptr(dst.contiguous()), src.numel(),
-                _lib.stream_ptr())
+        if max(sizes) >= 1 << 31:
+            raise ValueError("copy_pages: a page of 2 GB or more")
+        with _lib.on_device(device):
+            rc = _lib.entry("cb_beam_copy", "ppippip")(
+                (ctypes.c_void_p * n)(*base), (ctypes.c_int * n)(*sizes), n,
+                src.contiguous().data_ptr(), dst.contiguous().data_ptr(), src.numel(),
+                _lib.stream_int())
         _lib.check_rc(rc, "cb_beam_copy", launches=(n + 191) // 192)
         return
     for s, d in zip(src.tolist(), dst.tolist()):

@@ -48,54 +48,66 @@ def kv8_alloc(num_pages: int, heads: int, dh: int, kind: str, device
 
 
 def _check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, ints, row0, max_rows):
-    """Shapes and types of what every call takes; returns ``(pages, heads, dh)``."""
-    if k_cache.dim() != 5 or k_cache.shape[3:] != (PAGE, 64) or k_cache.dtype not in _QMAX:
+    """Shapes and types of what every call takes; returns ``(pages, heads, dh, entries, device)``, the
+    device as a number (-1: CPU)."""
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 5 or shape[3] != PAGE or shape[4] != 64 or dtype not in _QMAX:
         raise ValueError(f"{what}: keys are [pages, heads, dh / 64, {PAGE}, 64] codes, got "
-                         f"{tuple(k_cache.shape)} {k_cache.dtype}")
-    pages, heads, dh = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2] * 64
-    if dh not in (64, 128):
+                         f"{tuple(shape)} {dtype}")
+    pages, heads, dh = shape[0], shape[1], shape[2] * 64
+    if dh != 64 and dh != 128:
         raise ValueError(f"{what}: heads of 64 or 128, not {dh}")
-    if tuple(v_cache.shape) != (pages, heads, dh, PAGE) or v_cache.dtype != k_cache.dtype:
+    if v_cache.shape != (pages, heads, dh, PAGE) or v_cache.dtype != dtype:
         raise ValueError(f"{what}: values {tuple(v_cache.shape)} {v_cache.dtype} do not go with "
-                         f"keys {tuple(k_cache.shape)} {k_cache.dtype}")
-    for s in (k_scale, v_scale):
-        if tuple(s.shape) != (pages, heads) or s.dtype != torch.float32:
-            raise ValueError(f"{what}: scales are fp32 [{pages}, {heads}]")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1:
+                         f"keys {tuple(shape)} {dtype}")
+    if k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads) \
+            or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise ValueError(f"{what}: scales are fp32 [{pages}, {heads}]")
+    table = page_table.shape
+    if len(table) != 2 or table[1] < 1 or page_table.dtype != torch.int32:
         raise ValueError(f"{what}: the page table is int32 [entries, pages]")
-    n = page_table.shape[0]
-    if tuple(ints.shape) != (n,) or ints.dtype != torch.int32:
+    n = table[0]
+    if ints.shape != (n,) or ints.dtype != torch.int32:
         raise ValueError(f"{what}: one int32 number per entry, got {tuple(ints.shape)} {ints.dtype}")
-    if row0 is not None and (tuple(row0.shape) != (n + 1,) or row0.dtype != torch.int32):
-        raise ValueError(f"{what}: row0 is int32 [{n + 1}]")
+    given = (v_cache, k_scale, v_scale, page_table, ints)
+    if row0 is not None:
+        if row0.shape != (n + 1,) or row0.dtype != torch.int32:
+            raise ValueError(f"{what}: row0 is int32 [{n + 1}]")
+        given += (row0,)
     if max_rows < 1 or (row0 is None and max_rows != 1):
         raise ValueError(f"{what}: max_rows is the bound on an entry's rows (1 without row0)")
-    for t in (k_cache, v_cache, k_scale, v_scale, page_table, ints, row0):
-        if t is None:
-            continue
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: cache, tables and lengths have to be contiguous")
-        if t.is_cuda and t.data_ptr() % 16 and t.dim() > 2:
-            raise ValueError(f"{what}: the cache has to start at a multiple of 16 bytes")
-        if t.device != k_cache.device:
+    device = k_cache.get_device()
+    ok = k_cache.is_contiguous()
+    for t in given:
+        ok = ok and t.is_contiguous()
+        if t.get_device() != device:
             raise ValueError(f"{what}: tensors on {t.device} and {k_cache.device}")
-    return pages, heads, dh
+    if not ok:
+        raise ValueError(f"{what}: cache, tables and lengths have to be contiguous")
+    if device >= 0 and (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError(f"{what}: the cache has to start at a multiple of 16 bytes")
+    return pages, heads, dh, n, device
 
 
-def _rows(what: str, x: torch.Tensor, width: int, like: torch.Tensor) -> torch.Tensor:
+def _rows(what: str, x: torch.Tensor, width: int, device: int) -> torch.Tensor:
     """A row-wise input as the kernels read it: bf16, unit inner stride, 16-byte rows (a copy where
     the caller's view is laid out otherwise)."""
     if x.dim() != 2 or x.shape[1] != width:
         raise ValueError(f"{what}: rows of {width} numbers, got {tuple(x.shape)}")
-    if x.device != like.device:
-        raise ValueError(f"{what}: tensors on {x.device} and {like.device}")
-    if not x.is_cuda:
+    if x.get_device() != device:
+        raise ValueError(f"{what}: rows on {x.device}, the cache elsewhere")
+    if device < 0:
         return x
     if x.dtype != torch.bfloat16:
         raise ValueError(f"{what}: the kernels take bf16 rows, got {x.dtype}")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16 or x.stride(0) >= 1 << 31:
+    step = x.stride(0)
+    if x.stride(1) != 1 or step % 8 or x.data_ptr() % 16 or not 0 <= step < 1 << 31:
         x = x.contiguous()
     return x
+
+
+def _status(device: int) -> int:
+    return _lib.status_buffer(torch.device("cuda", device)).data_ptr()
 
 
 def _spans(n: int, row0, rows: int, max_rows: int):
@@ -153,25 +165,25 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     """Stores the rows of ``k`` / ``v`` (``[rows, heads * dh]`` views) at positions ``pos0[e]`` and on of
     each entry.  Tokens of the first page before ``pos0[e]`` are kept; what the page held from there on
     is not counted on any more."""
-    pages, heads, dh = _check("kv8_write", k_cache, v_cache, k_scale, v_scale, page_table, pos0,
-                              row0, max_rows)
-    k = _rows("kv8_write", k, heads * dh, k_cache)
-    v = _rows("kv8_write", v, heads * dh, k_cache)
-    if k.shape[0] != v.shape[0]:
-        raise ValueError(f"kv8_write: {k.shape[0]} rows of keys, {v.shape[0]} of values")
-    n, rows = page_table.shape[0], k.shape[0]
+    pages, heads, dh, n, device = _check("kv8_write", k_cache, v_cache, k_scale, v_scale,
+                                         page_table, pos0, row0, max_rows)
+    k = _rows("kv8_write", k, heads * dh, device)
+    v = _rows("kv8_write", v, heads * dh, device)
+    rows = k.shape[0]
+    if rows != v.shape[0]:
+        raise ValueError(f"kv8_write: {rows} rows of keys, {v.shape[0]} of values")
     if row0 is None and n > rows:
         raise ValueError(f"kv8_write: {n} entries, {rows} rows")
     if n == 0 or rows == 0:
         return
-    if k.is_cuda:
-        with torch.cuda.device(k.device):
-            rc = _lib.lib().cb_kv8_write(
-                _lib.ptr(k), _lib.ptr(v), k.stride(0), v.stride(0), _lib.ptr(k_cache),
-                _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale), _lib.ptr(page_table),
+    if device >= 0:
+        with _lib.on_device(device):
+            rc = _lib.entry("cb_kv8_write", "ppiippppp" + "iiiii" + "ppiiipp")(
+                k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k_cache.data_ptr(),
+                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
                 page_table.shape[1], pages, heads, dh, int(k_cache.dtype != torch.int8),
-                _lib.ptr(row0), _lib.ptr(pos0), n, rows, max_rows,
-                _lib.ptr(_lib.status_buffer(k.device)), _lib.stream_ptr())
+                None if row0 is None else row0.data_ptr(), pos0.data_ptr(), n, rows, max_rows,
+                _status(device), _lib.stream_int())
         _lib.check_rc(rc, "cb_kv8_write")
         return
     dtype = k_cache.dtype
@@ -212,25 +224,25 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
     """The stored keys and values of positions ``pos0[e]`` and on as ``[rows, heads * dh]`` (``dtype``;
     bf16 on a GPU, where it holds every stored value exactly).  ``rows`` is ``row0[n]``, known on the
     host; rows that no entry owns are not set."""
-    pages, heads, dh = _check("kv8_read", k_cache, v_cache, k_scale, v_scale, page_table, pos0,
-                              row0, max_rows)
+    pages, heads, dh, n, device = _check("kv8_read", k_cache, v_cache, k_scale, v_scale,
+                                         page_table, pos0, row0, max_rows)
     if row0 is None or rows < 0:
         raise ValueError("kv8_read: needs row0 and the number of rows")
-    n = page_table.shape[0]
-    if k_cache.is_cuda:
+    if device >= 0:
         if dtype != torch.bfloat16:
             raise ValueError(f"kv8_read: the kernels give bf16, not {dtype}")
         out = torch.empty((2, rows, heads * dh), dtype=dtype, device=k_cache.device)
+        k, v = out.unbind(0)
         if n and rows:
-            with torch.cuda.device(k_cache.device):
-                rc = _lib.lib().cb_kv8_read(
-                    _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale),
-                    _lib.ptr(page_table), page_table.shape[1], pages, heads, dh,
-                    int(k_cache.dtype != torch.int8), _lib.ptr(row0), _lib.ptr(pos0), n, rows,
-                    max_rows, _lib.ptr(out[0]), _lib.ptr(out[1]), heads * dh,
-                    _lib.ptr(_lib.status_buffer(k_cache.device)), _lib.stream_ptr())
+            with _lib.on_device(device):
+                rc = _lib.entry("cb_kv8_read", "ppppp" + "iiiii" + "ppiiippipp")(
+                    k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                    v_scale.data_ptr(), page_table.data_ptr(), page_table.shape[1], pages, heads,
+                    dh, int(k_cache.dtype != torch.int8), row0.data_ptr(), pos0.data_ptr(), n,
+                    rows, max_rows, k.data_ptr(), v.data_ptr(), heads * dh, _status(device),
+                    _lib.stream_int())
             _lib.check_rc(rc, "cb_kv8_read")
-        return out[0], out[1]
+        return k, v
     out = torch.zeros((2, rows, heads * dh), dtype=dtype)
     for e, r0, cnt in _spans(n, row0, rows, max_rows):
         at = int(pos0[e])
@@ -260,33 +272,34 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     are the last of them and every row sees the tokens up to itself; a row that sees none gets zeros, and
     so do rows that no entry owns.  Query head ``h`` reads cache head ``h // (nh // heads)``; ``scale``
     defaults to ``1 / sqrt(dh)``."""
-    pages, heads, dh = _check("kv8_attention", k_cache, v_cache, k_scale, v_scale, page_table,
-                              ctx_len, row0, max_rows)
+    pages, heads, dh, n, device = _check("kv8_attention", k_cache, v_cache, k_scale, v_scale,
+                                         page_table, ctx_len, row0, max_rows)
     if nh < 1 or nh % heads:
         raise ValueError(f"kv8_attention: {nh} query heads over {heads}")
-    q = _rows("kv8_attention", q, nh * dh, k_cache)
-    n, rows = page_table.shape[0], q.shape[0]
+    q = _rows("kv8_attention", q, nh * dh, device)
+    rows = q.shape[0]
     if row0 is None and n > rows:
         raise ValueError(f"kv8_attention: {n} entries, {rows} rows")
-    scale = scale if scale is not None else 1.0 / math.sqrt(dh)
-    if not 0.0 <= scale < math.inf:
+    if scale is None:
+        scale = 1.0 / math.sqrt(dh)
+    elif not 0.0 <= scale < math.inf:
         raise ValueError(f"kv8_attention: scale {scale}")
-    if q.is_cuda:
+    if device >= 0:
         whole = row0 is None and n == rows           # every row is written
         out = (torch.empty if whole else torch.zeros)((rows, nh * dh), dtype=torch.bfloat16,
                                                       device=q.device)
         if n == 0 or rows == 0:
             return out
-        with torch.cuda.device(q.device):
-            scratch = torch.empty(_scratch(n, rows, max_rows, nh // heads,
-                                           page_table.shape[1], heads, dh), dtype=torch.uint8,
-                                  device=q.device)
-            rc = _lib.lib().cb_kv8_attn(
-                _lib.ptr(q), q.stride(0), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale),
-                _lib.ptr(v_scale), _lib.ptr(page_table), page_table.shape[1], pages, heads, dh,
-                int(k_cache.dtype != torch.int8), _lib.ptr(ctx_len), _lib.ptr(row0), n, rows,
-                max_rows, nh, ctypes.c_float(scale), _lib.ptr(out), out.stride(0),
-                _lib.ptr(scratch), _lib.ptr(_lib.status_buffer(q.device)), _lib.stream_ptr())
+        width = page_table.shape[1]
+        with _lib.on_device(device):
+            scratch = torch.empty(_scratch(n, rows, max_rows, nh // heads, width, heads, dh),
+                                  dtype=torch.uint8, device=q.device)
+            rc = _lib.entry("cb_kv8_attn", "pippppp" + "iiiii" + "ppiiiifpippp")(
+                q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+                k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), width, pages, heads,
+                dh, int(k_cache.dtype != torch.int8), ctx_len.data_ptr(),
+                None if row0 is None else row0.data_ptr(), n, rows, max_rows, nh, scale,
+                out.data_ptr(), nh * dh, scratch.data_ptr(), _status(device), _lib.stream_int())
         _lib.check_rc(rc, "cb_kv8_attn", launches=2 * ((n + 255) // 256))
         return out
     out = torch.zeros((rows, nh * dh), dtype=q.dtype)

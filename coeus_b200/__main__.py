@@ -257,6 +257,12 @@ def _load_tokenizer(store, weights: str):
     return BpeTokenizer.load(str(path))
 
 
+def _kv_dtype(store) -> dict:
+    """``--kv_dtype=int8|e4m3``: the engine's cache in 8 bits."""
+    kind = _get(store, "kv_dtype")
+    return {} if not kind else {"kv_dtype": str(kind)}
+
+
 def cmd_generate(store, rest: List[str]) -> dict:
     import torch
 
@@ -276,10 +282,20 @@ def cmd_generate(store, rest: List[str]) -> dict:
         raise SystemExit("generate needs --prompt_ids=1,2,3, or --prompt=text with a tokenizer "
                          "file (<weights>.tokenizer.json or --tokenizer=...)")
     n = int(_get(store, "max_tokens") or 16)
-    out = make_engine(model, max_batch=1).generate(
-        torch.tensor(ids, device=device)[None], n,
-        temperature=float(_get(store, "temperature") or 0.0))
-    res = {"prompt_ids": ids, "token_ids": out[0, len(ids):].tolist()}
+    beams = int(_get(store, "beams") or 1)
+    engine = make_engine(model, max_batch=beams, **_kv_dtype(store))
+    prompt = torch.tensor(ids, device=device)[None]
+    if beams > 1:
+        eos = _get(store, "eos_id")
+        penalty = _get(store, "length_penalty")
+        found, scores = engine.beam_search(prompt, beams, n,
+                                           eos_id=None if eos is None else int(eos),
+                                           length_penalty=1.0 if penalty is None else float(penalty))
+        res = {"prompt_ids": ids, "token_ids": found[0, 0, len(ids):].tolist(),
+               "score": float(scores[0, 0])}
+    else:
+        out = engine.generate(prompt, n, temperature=float(_get(store, "temperature") or 0.0))
+        res = {"prompt_ids": ids, "token_ids": out[0, len(ids):].tolist()}
     if tok is not None:
         from .serve.server import _decoder
         res["text"] = _decoder(tok)(res["token_ids"])
@@ -358,6 +374,9 @@ def cmd_serve(store) -> int:
             loop = ServingLoop(None, engine=engine, group=group, **kw)
             loop.join()
             return 0
+    elif _kv_dtype(store):
+        from .infer.engine import make_engine
+        engine = make_engine(model, max_batch=max_seqs, **_kv_dtype(store))
     import uvicorn
     app = create_app(model, tokenizer=_load_tokenizer(store, str(weights) if weights else ""),
                      prefix_cache=bool(_get(store, "prefix_cache")), engine=engine, group=group,

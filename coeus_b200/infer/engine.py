@@ -7,16 +7,18 @@ token and returns one position."""
 from __future__ import annotations
 
 import time
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
 from ..foundation.error import ProcessingError
 from ..models.decoder import DecoderLM
 from ..ops import attention as A
+from ..ops import beam
 from ..ops import decode as D
 from ..ops import elementwise as E
 from ..ops import gemm as G
+from ..ops import kv8
 from ..ops import norm as N
 from ..ops import ring as R
 from .kv_cache import PagedKVCache
@@ -33,12 +35,20 @@ class InferenceEngine:
     ragged = False       # whether step() runs unequal entries as one batch
 
     def __init__(self, model: DecoderLM, max_batch: int = 64, max_len: Optional[int] = None,
-                 decode_splits: int = 0, use_graph: Optional[bool] = None) -> None:
+                 decode_splits: int = 0, use_graph: Optional[bool] = None,
+                 kv_dtype: Optional[str] = None) -> None:
         """``use_graph``: capture the decode step in a CUDA graph and replay it per token (default:
         on for CUDA models whose positions are not taken from a host-indexed table).  Positions
-        then live in device buffers that are never reallocated."""
+        then live in device buffers that are never reallocated.  ``kv_dtype``: ``"int8"`` or
+        ``"e4m3"`` keeps the cache in 8 bits (heads of 64 or 128), half the bytes that a token reads;
+        a prompt's own attention still sees its keys and values as computed."""
         self.m = model
         self.cfg = model.cfg
+        if kv_dtype is not None and (kv_dtype not in kv8.KINDS or
+                                     model.cfg.head_dim not in (64, 128)):
+            raise ProcessingError.unsupported(f"kv_dtype {kv_dtype!r}",
+                                              f"{' or '.join(kv8.KINDS)}, heads of 64 or 128")
+        self.kv_dtype = kv_dtype
         self.max_batch = max_batch
         self.max_len = max_len or self.cfg.max_seq_len
         self.decode_splits = decode_splits
@@ -57,16 +67,20 @@ class InferenceEngine:
         c = self.cache
         need_pages = (total + D.PAGE - 1) // D.PAGE
         if c is None or c.page_table.shape[0] < B or c.page_table.shape[1] < need_pages:
-            c = PagedKVCache.for_model(self.cfg, max(B, 1), max(total, D.PAGE), self.m.device)
-            if self.m.p16.dtype != torch.bfloat16:       # CPU oracle runs keep their precision
-                c.k = [t.to(self.m.p16.dtype) for t in c.k]
-                c.v = [t.to(self.m.p16.dtype) for t in c.v]
-            self.cache = c
+            c = PagedKVCache.for_model(self.cfg, max(B, 1), max(total, D.PAGE), self.m.device,
+                                       kind=self.kv_dtype)
+            self.cache = self._own_precision(c)
             self._graph = None
         for b in list(c.owned):
             c.release(b)
         for b in range(B):
             c.reserve(b, total)
+        return c
+
+    def _own_precision(self, c: PagedKVCache) -> PagedKVCache:
+        if c.kind is None and self.m.p16.dtype != torch.bfloat16:
+            c.k = [t.to(self.m.p16.dtype) for t in c.k]   # CPU oracle runs keep their precision
+            c.v = [t.to(self.m.p16.dtype) for t in c.v]
         return c
 
     def _norm(self, x, prefix):
@@ -89,14 +103,21 @@ class InferenceEngine:
                 cache: PagedKVCache, prefill: bool, pos_dev: Optional[torch.Tensor] = None,
                 page_table: Optional[torch.Tensor] = None,
                 earlier: Optional[List[list]] = None,
-                ctx: Optional[torch.Tensor] = None) -> torch.Tensor:
+                ctx: Optional[torch.Tensor] = None,
+                row0: Optional[torch.Tensor] = None, max_rows: int = 1) -> torch.Tensor:
         """``earlier[l]`` (chunked prefill) lists the ``(k, v)`` of the sequence chunks that came
-        before this one; this chunk attends to them without a mask, to itself causally, and the
-        partial results are merged by their log-sum-exp."""
+        before this one (with a cache in 8 bits their first positions: they are read back from it);
+        this chunk attends to them without a mask, to itself causally, and the
+        partial results are merged by their log-sum-exp.  With ``row0`` (cache in 8 bits only) the rows
+        are those of entries of up to ``max_rows`` tokens each, at positions ``pos_dev`` of their own, and
+        attend to the cache."""
         m, cfg = self.m, self.cfg
-        page_table = cache.page_table if page_table is None else page_table
+        page_table = cache.page_table[:B] if page_table is None else page_table
         H, nh, dh = cfg.hidden_dim, cfg.num_heads, cfg.head_dim
         n1n, n2n, _ = m.layout.norm_names
+        rows8 = row0             # 8 bits: the rows of every sequence
+        if cache.kind is not None and row0 is None and (S > 1 or earlier is not None):
+            rows8, max_rows = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=x.device), S
         for l in range(cfg.num_layers):
             p = f"layers.{l}."
             bias = (lambda n: m.w[p + n]) if cfg.use_bias else (lambda n: None)
@@ -112,7 +133,10 @@ class InferenceEngine:
             q, k, v = qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:]
             # grouped-query attention: the cache keeps the key/value heads as they are, the
             # prefill and decode kernels index them by query head // group
-            D.kv_write(k, v, cache.k[l], cache.v[l], page_table, pos0, S, cfg.kv_heads, dh)
+            if cache.kind is not None:
+                kv8.kv8_write(k, v, *cache.layer(l), page_table, pos0, rows8, max_rows)
+            else:
+                D.kv_write(k, v, cache.k[l], cache.v[l], page_table, pos0, S, cfg.kv_heads, dh)
             if prefill:
                 attn, lse = A.attention_fwd(q, k, v, B, S, nh, dh, causal=True)
                 if earlier is not None:
@@ -120,11 +144,17 @@ class InferenceEngine:
                         acc = torch.empty((B * S, H), dtype=torch.float32, device=x.device)
                         lse_acc = torch.empty_like(lse)
                         R.merge_partial(acc, lse_acc, attn, lse, B, S, nh, dh, True)
-                        for kj, vj in earlier[l]:
+                        for e in earlier[l]:
+                            kj, vj = e if cache.kind is None else kv8.kv8_read(
+                                *cache.layer(l), page_table, torch.full_like(pos0, e), rows8,
+                                B * S, S, dtype=k.dtype)
                             o_p, lse_p = A.attention_fwd(q, kj, vj, B, S, nh, dh, causal=False)
                             R.merge_partial(acc, lse_acc, o_p, lse_p, B, S, nh, dh, False)
                         R.cast_rows(acc, attn)
-                    earlier[l].append((k, v))
+                    earlier[l].append((k, v) if cache.kind is None else pos0_host)
+            elif cache.kind is not None:
+                attn = kv8.kv8_attention(q, *cache.layer(l), page_table,
+                                         self._ctx if ctx is None else ctx, nh, row0, max_rows)
             else:
                 attn = D.decode_attention(q, cache.k[l], cache.v[l], page_table,
                                           self._ctx if ctx is None else ctx, nh, dh,
@@ -153,6 +183,19 @@ class InferenceEngine:
         if B > self.max_batch:
             raise ProcessingError.limit_exceeded("batch size", self.max_batch, B)
         cache = self._ensure_cache(B, total_len)
+        last = self._prompts(ids, cache, cache.page_table, total_len, seq_chunk, token_chunk)
+        self._pos = S
+        self._pos0, self._ctx = self._pos_buf[:B], self._ctx_buf[:B]
+        self._pos0.fill_(S)
+        self._ctx.fill_(S)
+        return self._logits(last)
+
+    def _prompts(self, ids: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
+                 total_len: int, seq_chunk: Optional[int], token_chunk: Optional[int]
+                 ) -> torch.Tensor:
+        """The prompts through the model into the pages of ``page_table``'s rows; the last positions'
+        hidden states ``[B, H]``."""
+        B, S = ids.shape
         m, cfg = self.m, self.cfg
         nb = B if not seq_chunk else max(1, min(B, int(seq_chunk)))
         Sc = S
@@ -163,7 +206,7 @@ class InferenceEngine:
         for b0 in range(0, B, nb):
             b1 = min(B, b0 + nb)
             Bg = b1 - b0
-            table = cache.page_table[b0:b1]
+            table = page_table[b0:b1]
             earlier = [[] for _ in range(cfg.num_layers)] if Sc < S else None
             for c0 in range(0, S, Sc):
                 pos0 = torch.full((Bg,), c0, dtype=torch.int32, device=m.device)
@@ -172,11 +215,7 @@ class InferenceEngine:
                 x = self._layers(x, Bg, Sc, pos0, c0, cache, prefill=True, page_table=table,
                                  earlier=earlier)
             last[b0:b1] = x.view(Bg, Sc, -1)[:, -1, :]
-        self._pos = S
-        self._pos0, self._ctx = self._pos_buf[:B], self._ctx_buf[:B]
-        self._pos0.fill_(S)
-        self._ctx.fill_(S)
-        return self._logits(last)
+        return last
 
     # ------------------------------------------------------------------ slot-wise API (serving)
     def open_slots(self, max_seqs: int, max_len: int, num_pages: Optional[int] = None
@@ -186,14 +225,12 @@ class InferenceEngine:
         a pool of ``num_pages`` (default: enough for every slot to grow to ``max_len``)."""
         if num_pages is None:
             c = PagedKVCache.for_model(self.cfg, max_seqs, max(max_len, D.PAGE) + D.PAGE,
-                                       self.m.device)
+                                       self.m.device, kind=self.kv_dtype)
         else:
             c = PagedKVCache(self.cfg.num_layers, self.cfg.kv_heads, self.cfg.head_dim, num_pages,
-                             max_seqs, max(1, (max_len + D.PAGE - 1) // D.PAGE), self.m.device)
-        if self.m.p16.dtype != torch.bfloat16:       # CPU oracle runs keep their precision
-            c.k = [t.to(self.m.p16.dtype) for t in c.k]
-            c.v = [t.to(self.m.p16.dtype) for t in c.v]
-        self.cache = c
+                             max_seqs, max(1, (max_len + D.PAGE - 1) // D.PAGE), self.m.device,
+                             kind=self.kv_dtype)
+        self.cache = c = self._own_precision(c)
         self._graph = None
         return c
 
@@ -232,8 +269,12 @@ class InferenceEngine:
         P = len(prefix_pages) * PG
         if not 0 <= P < S:
             raise ProcessingError.invalid_input("the cached prefix must be shorter than the prompt")
-        H = cfg.hidden_dim
         cache.adopt(slot, list(prefix_pages))
+        if cache.kind is not None:       # the rest as one entry of many rows, on top of the pages
+            cache.reserve(slot, total_len)
+            x = self._entries([slot], [ids[P:]], [P])
+            cache.set_length(slot, S)
+            return self._logits(x[-1:].contiguous())[0]
         padded = P + (S - P + PG - 1) // PG * PG
         cache.reserve(slot, max(total_len, padded))
         pe = m._positions(max(padded, total_len))
@@ -271,12 +312,49 @@ class InferenceEngine:
                          ctx=ctx)
         return self._logits(x)
 
+    def _entries(self, slots: List[int], tokens: List[torch.Tensor], pos0: List[int]
+                 ) -> torch.Tensor:
+        """Hidden states of the tokens of several sequences in one pass over a cache in 8 bits: entry
+        ``i`` feeds ``tokens[i]`` (int64) at positions ``pos0[i]`` and on of cache row ``slots[i]``."""
+        cache, m, cfg = self.cache, self.m, self.cfg
+        dev = m.device
+        n = [int(t.numel()) for t in tokens]
+        row0 = [0]
+        for c in n:
+            row0.append(row0[-1] + c)
+        place = torch.tensor([p + t for p, c in zip(pos0, n) for t in range(c)], dtype=torch.int32,
+                             device=dev)
+        meta = torch.tensor([pos0, [p + c for p, c in zip(pos0, n)]], dtype=torch.int32, device=dev)
+        x = E.embed_fwd(torch.cat(tokens), m.w["token_embed"], None, 1)
+        if cfg.pos in ("sinusoidal", "learned"):
+            pe = m._positions(max(p + c for p, c in zip(pos0, n)))
+            x = (x.float() + pe[place.long()].float()).to(x.dtype)
+        table = cache.page_table.index_select(
+            0, torch.tensor(slots, dtype=torch.int64, device=dev))
+        return self._layers(x, row0[-1], 1, meta[0], 0, cache, prefill=False,
+                            pos_dev=place if cfg.pos == "rope" else None, page_table=table,
+                            ctx=meta[1], row0=torch.tensor(row0, dtype=torch.int32, device=dev),
+                            max_rows=max(n))
+
     def step(self, entries) -> Optional[torch.Tensor]:
         """The next tokens of several sequences (:class:`coeus_b200.ops.ragged.Entry`), cut anywhere;
-        the logits ``[wanted, V]`` of the wanted places in order.  This decoder's kernels want one
+        the logits ``[wanted, V]`` of the wanted places in order.  Over a cache in 8 bits they run as one
+        batch; the attention over the bf16 cache wants one
         token per sequence, so an entry's tokens take one decode batch each."""
         for e in entries:
             self.cache.reserve(e.slot, e.pos0 + len(e.tokens))
+        if self.cache.kind is not None:
+            x = self._entries([e.slot for e in entries],
+                              [torch.tensor(e.tokens, dtype=torch.int64, device=self.m.device)
+                               for e in entries], [e.pos0 for e in entries])
+            want, at = [], 0
+            for e in entries:
+                self.cache.set_length(e.slot, e.pos0 + len(e.tokens))
+                want += [at + k for k in e.want]
+                at += len(e.tokens)
+            if not want:
+                return None
+            return self._logits(x[torch.tensor(want, dtype=torch.int64, device=x.device)])
         got = {}
         for k in range(max(len(e.tokens) for e in entries)):
             live = [(i, e) for i, e in enumerate(entries) if k < len(e.tokens)]
@@ -385,3 +463,123 @@ class InferenceEngine:
                       "prefill_tokens_per_s": B * S / max(t1 - t0, 1e-9),
                       "decode_tokens_per_s": B * max(0, max_new_tokens - 1) / max(t2 - t1, 1e-9)}
         return out
+
+    # ------------------------------------------------------------------ beam search
+    def beam_search(self, ids: torch.Tensor, beams: int, max_new_tokens: int,
+                    eos_id: Optional[int] = None, length_penalty: float = 1.0,
+                    keep: int = 1, seq_chunk: Optional[int] = None,
+                    token_chunk: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The ``keep`` best of ``beams`` continuations of every prompt of ``ids [B, S]``: token ids ``[B,
+        keep, S + max_new_tokens]`` (padded with ``eos_id`` behind it) and their scores ``[B, keep]``, the
+        summed log-probability divided by the number of new tokens (up to and with ``eos_id``) to the power
+        of ``length_penalty``.
+
+        A step selects the best continuations over all beams of a request
+        (:func:`coeus_b200.ops.beam.beam_select`) and moves the beams' cache pages to where their parents'
+        are (:func:`~coeus_b200.ops.beam.beam_reorder`): the prompt and what beams have in common is held
+        once, and only a page that is not full is ever copied.  Ended beams stay where they are."""
+        if ids.dim() == 1:
+            ids = ids[None]
+        B, S = ids.shape
+        m, cfg, dev = self.m, self.cfg, self.m.device
+        K, total, V = int(beams), S + int(max_new_tokens), cfg.vocab_size
+        if not 1 <= K <= beam.MAX_BEAMS or not 1 <= keep <= K:
+            raise ProcessingError.invalid_input(
+                f"{beams} beams (up to {beam.MAX_BEAMS}), {keep} of them kept")
+        if B < 1 or S < 1 or max_new_tokens < 1:
+            raise ProcessingError.invalid_input("beam search needs a prompt and a token to find")
+        if B * K > self.max_batch:
+            raise ProcessingError.limit_exceeded("beams of a batch", self.max_batch, B * K)
+        if total > max(self.max_len, cfg.max_seq_len) and cfg.pos != "rope":
+            raise ProcessingError.limit_exceeded("sequence length", cfg.max_seq_len, total)
+        if eos_id is not None and not 0 <= eos_id < V:
+            raise ProcessingError.invalid_input(f"eos_id {eos_id} is outside the vocabulary of {V}")
+        PG = D.PAGE
+        width = total // PG + 1
+        prompt_pages = (S + PG - 1) // PG
+        own = K * (width - S // PG + 1)           # pages that a request's beams may need beside these
+        cache = self._own_precision(PagedKVCache(
+            cfg.num_layers, cfg.kv_heads, cfg.head_dim, B * (prompt_pages + own), B * K, width, dev,
+            kind=self.kv_dtype))
+        pages = torch.arange(B * (prompt_pages + own), dtype=torch.int32, device=dev).view(B, -1)
+        pool = pages[:, prompt_pages:].contiguous()
+        table = cache.page_table
+        table.view(B, K, width)[:, :, :prompt_pages] = pages[:, None, :prompt_pages]
+        last = self._prompts(ids, cache, table[::K].contiguous(), total, seq_chunk, token_chunk)
+        # the first step starts from one copy of the prompt
+        logits = self._logits(last)[:, :V].repeat_interleave(K, 0)
+        scores = torch.full((B, K), float("-inf"), device=dev)
+        scores[:, 0] = 0.0
+        done = torch.zeros((B, K), dtype=torch.bool, device=dev)
+        length = torch.full((B,), S, dtype=torch.int32, device=dev)
+        pos0 = torch.full((B * K,), S, dtype=torch.int32, device=dev)
+        ctx = pos0 + 1
+        tensors = cache.tensors()
+        parents, tokens = [], []
+
+        def advance(token: torch.Tensor, parent: torch.Tensor, pos: int) -> torch.Tensor:
+            """One token of every beam behind its parent, at position ``pos``; the logits."""
+            table.copy_(beam.beam_reorder(table, parent, length, pool, tensors))
+            token = token.reshape(-1)
+            if cfg.pos in ("sinusoidal", "learned"):
+                x = E.embed_fwd(token, m.w["token_embed"], m._positions(pos + 1), 1, pos_offset=pos)
+            else:
+                x = E.embed_fwd(token, m.w["token_embed"], None, 1)
+            x = self._layers(x, B * K, 1, pos0, pos, cache, prefill=False,
+                             pos_dev=pos0 if cfg.pos == "rope" else None, page_table=table, ctx=ctx)
+            length.add_(1)
+            pos0.add_(1)
+            ctx.add_(1)
+            return self._logits(x)[:, :V]
+
+        def step(logits: torch.Tensor, pos: int):
+            """Selection and the next token's logits, every state in place."""
+            new, parent, token, ended = beam.beam_select(logits, scores, done, eos_id)
+            scores.copy_(new)
+            done.copy_(ended)
+            return parent, token, advance(token, parent, pos)
+
+        graph = None
+        capture = self.use_graph and max_new_tokens > 3 and cfg.pos not in ("sinusoidal", "learned")
+        for i in range(max_new_tokens):
+            if i == max_new_tokens - 1:                    # nothing comes after the last selection
+                scores, parent, token, done = beam.beam_select(logits, scores, done, eos_id)
+            elif graph is not None:
+                graph[0].replay()
+                parent, token = graph[1].clone(), graph[2].clone()
+            elif capture and i == 1:
+                # the first pass was the warm-up; from here on every step is the same launches
+                held = logits.clone()
+                torch.cuda.synchronize(dev)
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    parent, token, out = step(held, S + i)
+                    held.copy_(out)
+                logits = held
+                graph = (g, parent, token)
+                g.replay()
+                parent, token = parent.clone(), token.clone()
+            else:
+                parent, token, logits = step(logits, S + i)
+            parents.append(parent)
+            tokens.append(token)
+            if eos_id is not None and i + 1 < max_new_tokens and bool(done.all()):
+                break
+        # back from the last selection to the first
+        n = len(tokens)
+        fill = eos_id if eos_id is not None else 0
+        found = torch.full((B, K, int(max_new_tokens)), fill, dtype=torch.int64, device=dev)
+        at = torch.arange(K, device=dev).expand(B, K)
+        for i in range(n - 1, -1, -1):
+            found[:, :, i] = torch.gather(tokens[i], 1, at)
+            at = torch.gather(parents[i], 1, at)
+        count = torch.full((B, K), n, dtype=torch.float32, device=dev)
+        if eos_id is not None:
+            hit = found[:, :, :n] == eos_id
+            first = hit.to(torch.int8).argmax(-1) + 1
+            count = torch.where(hit.any(-1), first.float(), count)
+        ranked = scores / count ** length_penalty
+        best, order = torch.sort(ranked, dim=1, descending=True, stable=True)
+        found = torch.gather(found, 1, order[:, :keep, None].expand(B, keep, found.shape[2]))
+        out = torch.cat([ids[:, None].expand(B, keep, S).to(torch.int64), found], -1)
+        return out, best[:, :keep]

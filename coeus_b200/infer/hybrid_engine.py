@@ -53,6 +53,7 @@ class HybridEngine(InferenceEngine):
                  use_graph: Optional[bool] = None) -> None:
         self.m = model
         self.cfg = model.cfg
+        self.kv_dtype = None         # every layer's cache is laid out on its own
         self.max_batch = max_batch
         self.max_len = max_len or self.cfg.max_seq_len
         self.cache: Optional[PagedKVCache] = None
@@ -85,6 +86,10 @@ class HybridEngine(InferenceEngine):
     def _batch(self, entries: List[Entry], into: Optional[R.RaggedBatch] = None) -> R.RaggedBatch:
         return R.RaggedBatch(entries, self.m.device, tile_rows=self._tiles, into=into,
                              plans=self._plans)
+
+    def beam_search(self, *args, **kw):
+        raise ProcessingError.unsupported(
+            "beam search with this model", "its layers carry state that cache pages do not hold")
 
     # ------------------------------------------------------------------ cache and state
     def open_slots(self, max_seqs: int, max_len: int, num_pages: Optional[int] = None

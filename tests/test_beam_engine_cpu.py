@@ -1,0 +1,171 @@
+"""Beam search and the 8-bit cache through the engine, the batcher and the command line, on the CPU."""
+import json
+import math
+
+import pytest
+import torch
+
+from coeus_b200.foundation.error import ProcessingError
+from coeus_b200.infer.engine import InferenceEngine
+from coeus_b200.infer.scheduler import ContinuousBatcher
+from coeus_b200.models.config import DecoderConfig
+from coeus_b200.models.decoder import DecoderLM
+from coeus_b200.ops.ragged import Entry
+
+
+def model(kind="llama", vocab=61, seed=0):
+    torch.manual_seed(seed)
+    kw = dict(hidden_dim=128, num_layers=2, num_heads=2, intermediate_dim=192, vocab_size=vocab,
+              max_seq_len=256)
+    if kind != "gpt":
+        kw.update(use_bias=False, activation="swiglu", norm="rmsnorm", pos="rope")
+    if kind == "gqa":
+        kw.update(num_heads=2, num_kv_heads=1)
+    m = DecoderLM(DecoderConfig(**kw), device="cpu", dtype=torch.float32, training=False)
+    for name, w in m.w.items():              # logits that are far from even
+        if name.endswith("embed") or "output" in name:
+            w.mul_(8.0)
+    return m
+
+
+def plain_beams(m, prompt, K, n, eos, penalty):
+    """Beam search by recomputing the whole sequence of every beam for every token."""
+    beams = [(0.0, [], False)]
+    for _ in range(n):
+        cand = []
+        for j, (s, toks, over) in enumerate(beams):
+            if over:
+                cand.append((-s, j, eos, toks + [eos], True))
+                continue
+            ids = torch.tensor([prompt + toks])
+            x = m.forward_logits(ids)[0, -1, :m.cfg.vocab_size].double()
+            lp = torch.log_softmax(x, -1)
+            top = torch.topk(lp, min(K, lp.numel()))
+            for v, t in zip(top.values.tolist(), top.indices.tolist()):
+                cand.append((-(s + v), j, t, toks + [t], t == eos))
+        cand.sort(key=lambda c: c[:3])
+        beams = [(-c[0], c[3], c[4]) for c in cand[:K]]
+        if all(b[2] for b in beams):
+            break
+    out = []
+    for s, toks, over in beams:
+        c = toks.index(eos) + 1 if eos is not None and eos in toks else len(toks)
+        out.append((s / c ** penalty, toks + [eos if eos is not None else 0] * (n - len(toks))))
+    out.sort(key=lambda o: -o[0])
+    return out
+
+
+@pytest.mark.parametrize("kind", ["gpt", "llama", "gqa"])
+@pytest.mark.parametrize("S,K,n,eos", [(5, 3, 6, None), (63, 4, 5, 7), (64, 2, 3, 7), (60, 1, 8, None)])
+def test_beam_search_against_full_recomputation(kind, S, K, n, eos):
+    m = model(kind)
+    g = torch.Generator().manual_seed(S)
+    ids = torch.randint(0, 61, (2, S), generator=g)
+    out, scores = InferenceEngine(m, max_batch=8).beam_search(ids, K, n, eos_id=eos, length_penalty=0.7, keep=K)
+    for b in range(2):
+        want = plain_beams(m, ids[b].tolist(), K, n, eos, 0.7)
+        for i in range(K):
+            assert out[b, i, :S].tolist() == ids[b].tolist()
+            assert out[b, i, S:].tolist() == want[i][1]
+            # sums of fp32 log-probabilities of a few tokens
+            assert abs(float(scores[b, i]) - want[i][0]) < 1e-4
+
+
+def test_one_beam_is_greedy_and_a_beam_beyond_pages():
+    m = model()
+    eng = InferenceEngine(m, max_batch=8)
+    ids = torch.randint(0, 61, (2, 50), generator=torch.Generator().manual_seed(1))
+    greedy = eng.generate(ids, 90)
+    out, _ = eng.beam_search(ids, 1, 90)
+    assert torch.equal(out[:, 0], greedy)
+    a, sa = eng.beam_search(ids, 4, 90, token_chunk=10)
+    b, sb = eng.beam_search(ids[1:], 4, 90)
+    assert torch.equal(a[1:], b) and torch.allclose(sa[1:], sb, atol=1e-4)
+    assert bool((a[:, 0] != greedy).any())         # looking ahead finds something else here
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("kind", ["gpt", "gqa"])
+def test_engine_with_8_bit_cache(kv, kind):
+    """One token at a time, several at once, on top of cached pages: the same numbers; and near those of
+    the cache that is not rounded."""
+    m = model(kind)
+    ids = torch.randint(0, 61, (1, 150), generator=torch.Generator().manual_seed(2))
+    eng = InferenceEngine(m, max_batch=4, kv_dtype=kv)
+    eng.open_slots(4, 256)
+    assert eng.cache.k[0].element_size() == 1
+    eng.prefill_slot(0, ids[0, :140], 160)
+    one = [eng.step([Entry(0, 140 + i, [int(ids[0, 140 + i])], [0])]) for i in range(10)]
+    eng.prefill_slot(1, ids[0, :140], 160)
+    many = eng.step([Entry(1, 140, ids[0, 140:].tolist(), list(range(10)))])
+    # a chunk's tokens share the scale of their page from the start; with powers of two that only
+    # moves where the smallest codes are rounded
+    assert torch.allclose(torch.cat(one), many, atol=2e-2, rtol=0)
+    pages = eng.cache.owned[0][:2]
+    top = eng.prefill_slot_paged(2, ids[0], 160, pages)
+    full = InferenceEngine(m, max_batch=4)
+    full.open_slots(4, 256)
+    want = full.prefill_slot(0, ids[0], 160)
+    size = float(want.abs().max())
+    for got in (many[-1], top):
+        assert float((got - want).abs().max()) < 0.08 * size
+    # chunks of a prompt read the earlier ones back
+    eng.cache.release(3)
+    a = eng.prefill_slot(3, ids[0], 160, token_chunk=50)
+    assert float((a - want).abs().max()) < 0.08 * size
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+def test_batcher_and_beams_over_8_bits(kv):
+    m = model("gqa")
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, 61, (n,), generator=g).tolist() for n in (70, 3, 130)]
+    alone = []
+    for p in prompts:
+        eng = InferenceEngine(m, max_batch=4, kv_dtype=kv)
+        alone.append(eng.generate(torch.tensor([p]), 12)[0, len(p):].tolist())
+    for prefix in (False, True):
+        b = ContinuousBatcher(InferenceEngine(m, max_batch=4, kv_dtype=kv), max_seqs=2, max_len=256,
+                              prefix_cache=prefix)
+        rids = [b.submit(p, 12) for p in prompts]
+        out = b.run()
+        if not prefix:
+            assert [out[r] for r in rids] == alone
+        again = b.submit(prompts[2], 12)
+        assert len(b.run()[again]) == 12
+    eng = InferenceEngine(m, max_batch=8, kv_dtype=kv)
+    one, _ = eng.beam_search(torch.tensor([prompts[0]]), 1, 12)
+    assert one[0, 0, 70:].tolist() == alone[0]
+    out, scores = eng.beam_search(torch.tensor([prompts[0]]), 4, 40, keep=4)
+    assert out.shape == (1, 4, 110) and bool((scores[0, :-1] >= scores[0, 1:]).all())
+    assert len({tuple(x) for x in out[0].tolist()}) == 4
+
+
+def test_refusals():
+    m = model()
+    eng = InferenceEngine(m, max_batch=4)
+    ids = torch.zeros((2, 5), dtype=torch.int64)
+    for kw in (dict(beams=0), dict(beams=3), dict(beams=33), dict(beams=2, keep=3), dict(beams=2, max_new_tokens=0),
+               dict(beams=2, eos_id=61)):
+        with pytest.raises(ProcessingError):
+            eng.beam_search(ids, **{"max_new_tokens": 3, **kw})
+    with pytest.raises(ProcessingError):
+        eng.beam_search(ids[:, :0], 2, 3)
+    with pytest.raises(ProcessingError):
+        InferenceEngine(m, kv_dtype="fp4")
+    small = DecoderLM(DecoderConfig(hidden_dim=64, num_layers=1, num_heads=2, intermediate_dim=64,
+                                    vocab_size=31, max_seq_len=64), device="cpu", training=False)
+    with pytest.raises(ProcessingError):
+        InferenceEngine(small, kv_dtype="int8")
+
+
+def test_command_line(tmp_path, capsys):
+    from coeus_b200.__main__ import main
+    from coeus_b200.checkpoint.formats import save_model
+    m = model("gpt")
+    path = tmp_path / "m.safetensors"
+    save_model(m, str(path))
+    main(["generate", f"--weights={path}", "--prompt_ids=5,6,7", "--max_tokens=6", "--beams=3",
+          "--kv_dtype=int8", "--device=cpu"])
+    out = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert len(out["token_ids"]) == 6 and math.isfinite(out["score"]) and out["score"] < 0.0

@@ -23,55 +23,21 @@
 // by its conversion.  Queries are fp16 after division by a power of two per row.  Weights enter the second product
 // as fp16 times 2^12: smaller than 2^-26 of the row's largest they start to lose bits, and less than 2^-36
 // of it is lost in all; the page's 2^ev is applied in fp32 to the sums of a page.
-#include "kv8.cuh"
+#include "kv8_attn.cuh"
 
 namespace cb {
 
 constexpr int KA_ROWS = 8;                        // query rows of a tile
-constexpr int KA_ENTRIES = 256;                   // of one launch
 constexpr int KA_SHARE = 2;                       // units a CTA takes at least
 constexpr int KA_EXTRA = 1;                       // what a tile costs beside its pages, in units
+// Rows and heads of an entry that share a key/value head: more take the wide tiles.  36 of them (24 sequences, 500 to
+// 4100 tokens): 86 us here, 98 us there; 2800: 1909 and 469.
+constexpr int KA_WIDE = 48;
 constexpr int KA_BLOCK = 16;                      // units that are planned at a time
 constexpr int KA_RING = 4;                        // copies in a warp's ring: the keys and values of two pages
 constexpr int KA_PLACES = 6, KA_PLACES64 = 11;    // CTAs that share an SM, by its shared memory: dh 128, 64
 constexpr float KA_SHIFT = 12.f;                  // weights are held times 2^12
 
-struct Kv8Desc {           // the tile that a CTA's run of units starts in
-  int lo, hi, share, units;
-  int entry, head, tile, pad;
-};
-
-struct Kv8Attn {
-  Kv8Cache c;
-  const __nv_bfloat16* q;  // [rows, ldq]
-  __nv_bfloat16* out;      // [rows, ldo]
-  int ldq, ldo, group;     // query heads per key/value head
-  const int* ctx;          // [entries]
-  const int* row0;         // [entries + 1] or null: entry e has row first + e alone
-  int first, n, rows, most;
-  float scale_log2;
-  float* part_o;           // [CTAs, 2, KA_ROWS, dh]
-  float* part_ml;          // [CTAs, 2, KA_ROWS, 2]
-  Kv8Desc* desc;           // [CTAs]
-  int* status;
-};
-
-// Four codes to two pairs of fp16.
-template <int KIND>
-__device__ __forceinline__ void kv8_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (KIND == KV8_INT8) {
-    const uint32_t x = w ^ 0x80808080u;                       // code + 128
-    lo = __byte_perm(x, 0x64646464u, 0x4140);                 // 1024 + that
-    hi = __byte_perm(x, 0x64646464u, 0x4342);
-    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
-    const __half2 p = __hsub2(*reinterpret_cast<__half2*>(&lo), off), q = __hsub2(*reinterpret_cast<__half2*>(&hi), off);
-    lo = *reinterpret_cast<const uint32_t*>(&p);
-    hi = *reinterpret_cast<const uint32_t*>(&q);
-  } else {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-  }
-}
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
       "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -83,48 +49,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// Wait for a phase, with a limit; the clock is asked only after many tries have failed.
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
-  const uint32_t at = smem_u32(bar);
-  uint64_t began = 0;
-  for (uint32_t n = 1;; ++n) {
-    if (mbar_try_wait(at, parity)) return true;
-    if (n % 256u == 0u) {
-      if (*abort_flag) return false;
-      const uint64_t now = globaltimer_ns();
-      if (began == 0) began = now;
-      else if (now - began > CB_WAIT_LIMIT_NS) {
-        *abort_flag = 1u;
-        return false;
-      }
-    }
-  }
-}
-
-// What one part of a softmax counts against the whole: its maximum m and sum l, the largest maximum.
-// A part without keys has m = -inf and l = 0; one whose scores are NaN has l = NaN, which stays.
-__device__ __forceinline__ float part_weight(float m, float l, float gm) {
-  if (m == -INFINITY) return l == 0.f ? 0.f : 1.f;
-  return fast_exp2(m - gm);
-}
-
-// Entry of a launch: rows and context as they are used; -1 rows if something is out of range.
-struct Kv8Entry {
-  int first, rows, ctx;
-};
-__device__ __forceinline__ Kv8Entry kv8_entry(const Kv8Attn& a, int e) {
-  Kv8Entry x;
-  x.first = a.row0 != nullptr ? a.row0[e] : a.first + e;
-  x.rows = a.row0 != nullptr ? a.row0[e + 1] - x.first : 1;
-  x.ctx = max(0, a.ctx[e]);
-  if (x.rows <= 0) x.rows = 0;
-  else if (x.rows > a.most || x.first < 0 || x.first + x.rows > a.rows) x.rows = -1;
-  return x;
-}
+// kv8_attn_rows.cu
+int launch_kv8_rows(const Kv8Attn& a, int kind, int dh, int ctas, cudaStream_t st);
+int kv8_rows_tile();
+int kv8_rows_share();
+int kv8_rows_extra();
 
 // A unit as it is planned: a page of a tile, and the tile's share of the CTA's units (counted from 0).
 struct Kv8Unit {
@@ -160,80 +89,16 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
   // ---- the plan: units before every entry
   if (lane == 0) {
     abort_flag = 0u;
-    prefix[0] = 0;
     for (int i = 0; i < RING; ++i) mbar_init(smem_u32(full + i), 1);
     mbar_fence_init();
   }
-  auto entry_of = [&](int e) {                                  // rows 0: nothing to do
-    Kv8Entry x = kv8_entry(a, e);
-    x.rows = max(x.rows, 0);
-    x.ctx = min(x.ctx, a.c.max_pages * KV8_PAGE);
-    return x;
-  };
-  int units = 0;
-#pragma unroll 4
-  for (int e0 = 0; e0 < a.n; e0 += 32) {
-    const int e = e0 + lane;
-    int s = 0;
-    if (e < a.n) {
-      const Kv8Entry x = entry_of(e);
-      if (blockIdx.x == 0 && (kv8_entry(a, e).rows < 0 || a.ctx[e] > a.c.max_pages * KV8_PAGE)) record_status(a.status, ST_BOUNDS, e);
-      if (x.ctx > 0) s = (x.rows * a.group + QR - 1) / QR * ((x.ctx + KV8_PAGE - 1) / KV8_PAGE + KA_EXTRA) * nkv;
-    }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += t;
-    }
-    if (e < a.n) prefix[e + 1] = units + s;
-    units += __shfl_sync(0xffffffffu, s, 31);
-  }
-  __syncwarp();
+  const int units = kv8_plan(a, QR, KA_EXTRA, prefix, lane);
   const int share = max((units - 1) / static_cast<int>(gridDim.x) + 1, KA_SHARE);
   const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(share) * blockIdx.x));
   const int u1 = min(units - u0, share) + u0, n_units = u1 - u0;
 
-  struct Where {           // a unit's tile
-    int e, hk, tile, pages;
-    int lo;                // its first unit
-    Kv8Entry x;
-  };
-  auto locate = [&](int u) {
-    int lo = 0, hi = a.n;                                       // prefix[lo] <= u < prefix[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= u) lo = mid;
-      else hi = mid;
-    }
-    Where w;
-    w.e = lo;
-    w.x = entry_of(lo);
-    w.pages = (w.x.ctx + KV8_PAGE - 1) / KV8_PAGE;
-    const int tiles = (w.x.rows * a.group + QR - 1) / QR, t = (u - prefix[lo]) / (w.pages + KA_EXTRA);
-    w.hk = t / tiles;
-    w.tile = t % tiles;
-    w.lo = prefix[lo] + t * (w.pages + KA_EXTRA);
-    return w;
-  };
-  if (lane == 0) {
-    Kv8Desc d{u0, u0, share, units, 0, 0, 0, 0};
-    if (n_units > 0) {
-      const Where w = locate(u0);
-      d.lo = w.lo;
-      d.hi = w.lo + w.pages;
-      d.entry = w.e;
-      d.head = w.hk;
-      d.tile = w.tile;
-    }
-    a.desc[blockIdx.x] = d;
-  }
-  // ---- entries without keys: their rows are zero
-  for (int e = blockIdx.x; e < a.n; e += gridDim.x) {
-    const Kv8Entry x = entry_of(e);
-    if (x.ctx == 0)
-      for (int r = 0; r < x.rows; ++r)
-        for (int i = lane; i < a.group * nkv * DH; i += 32) a.out[static_cast<size_t>(x.first + r) * a.ldo + i] = __float2bfloat16(0.f);
-  }
+  if (lane == 0) kv8_describe(a, QR, KA_EXTRA, prefix, u0, n_units, share, units);
+  kv8_zero_rows<DH>(a, lane, 32);
 
   const int g = lane >> 2, c = lane & 3;
   // Units are planned KA_BLOCK at a time, one a lane, while those before them run: what the page table and the scales
@@ -243,7 +108,7 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
     const int j = block * KA_BLOCK + lane;
     x.flags = 0;
     if (j >= n_units || lane >= KA_BLOCK) return;
-    const Where w = locate(u0 + j);
+    const Kv8Where w = kv8_locate(a, QR, KA_EXTRA, prefix, u0 + j);
     x.p = u0 + j - w.lo;
     if (x.p >= w.pages) return;
     x.flags = UNIT_PAGE;
@@ -537,73 +402,6 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
   }
 }
 
-// Tiles that lie in more than one CTA: the CTA behind the tile's first boundary has its block here.  The warps take the
-// parts in turn.
-constexpr int KM_WARPS = 16;
-template <int DH>
-__global__ void __launch_bounds__(32 * KM_WARPS) kv8_attn_merge_kernel(const __grid_constant__ Kv8Attn a) {
-  constexpr int QR = KA_ROWS, PER = DH / 32;
-  __shared__ float s_max[KM_WARPS], s_sum[KM_WARPS];
-  __shared__ float s_o[KM_WARPS][DH];
-  asm volatile("griddepcontrol.wait;" ::: "memory");             // the parts are complete
-  const int b = blockIdx.x + 1;
-  const Kv8Desc d = a.desc[b];
-  const long long at = static_cast<long long>(d.share) * b;
-  // starts here, ends before, or has begun before the last boundary
-  if (at >= d.units || d.lo >= at || d.hi <= at || d.lo < at - d.share) return;
-  const int parts = static_cast<int>((d.hi - at + d.share - 1) / d.share) + 1;
-  const size_t s0 = static_cast<size_t>(b - 1) * 2 + (d.lo == at - d.share ? 0 : 1);
-  auto slot = [&](int i) { return i == 0 ? s0 : static_cast<size_t>(b - 1 + i) * 2; };
-  const Kv8Entry x = kv8_entry(a, d.entry);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_rows = min(QR, x.rows * a.group - d.tile * QR);
-  const int ctx = min(x.ctx, a.c.max_pages * KV8_PAGE);
-  // warp w has row w mod n_rows, and of its parts every subs-th from w / n_rows on
-  const int r = warp % n_rows, sub = warp / n_rows, subs = KM_WARPS / n_rows;
-  const int mine = sub < subs && sub < parts ? (parts - sub + subs - 1) / subs : 0;
-  auto ml = [&](int i) { return *reinterpret_cast<const float2*>(a.part_ml + (slot(sub + subs * i) * QR + r) * 2); };
-  float gm = -INFINITY, gl = 0.f, o[PER];
-  for (int i = lane; i < mine; i += 32) gm = fmaxf(gm, ml(i).x);
-  gm = warp_max(gm);
-  if (lane == 0) s_max[warp] = gm;
-#pragma unroll
-  for (int y = 0; y < PER; ++y) o[y] = 0.f;
-  __syncthreads();
-  for (int w = r; w < subs * n_rows; w += n_rows) gm = fmaxf(gm, s_max[w]);
-  for (int i0 = 0; i0 < mine; i0 += 32) {
-    float k = 0.f;
-    if (i0 + lane < mine) {
-      const float2 v = ml(i0 + lane);
-      k = part_weight(v.x, v.y, gm);
-      if (k != 0.f) gl += k * v.y;
-    }
-    const int n = min(32, mine - i0);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float ki = __shfl_sync(0xffffffffu, k, i);
-      const float* src = a.part_o + (slot(sub + subs * (i0 + i)) * QR + r) * DH + lane * PER;
-#pragma unroll
-      for (int y = 0; y < PER; ++y) o[y] = fmaf(ki, src[y], o[y]);
-    }
-  }
-  gl = warp_sum(gl);
-  if (lane == 0) s_sum[warp] = gl;
-#pragma unroll
-  for (int y = 0; y < PER; ++y) s_o[warp][lane * PER + y] = o[y];
-  __syncthreads();
-  for (int e = threadIdx.x; e < n_rows * DH; e += 32 * KM_WARPS) {
-    const int er = e / DH, ch = e % DH, rr = d.tile * QR + er;
-    float v = 0.f, sum = 0.f;
-    for (int w = er; w < subs * n_rows; w += n_rows) {
-      v += s_o[w][ch];
-      sum += s_sum[w];
-    }
-    const bool any = ctx - x.rows + rr / a.group + 1 > 0;
-    a.out[static_cast<size_t>(x.first + rr / a.group) * a.ldo + (d.head * a.group + rr % a.group) * DH + ch] =
-        __float2bfloat16(any ? v / sum : 0.f);
-  }
-}
-
 template <int KIND, int DH>
 static int launch_attn(const Kv8Attn& a, int ctas, cudaStream_t st) {
   using S = Kv8Smem<DH>;
@@ -616,43 +414,40 @@ static int launch_attn(const Kv8Attn& a, int ctas, cudaStream_t st) {
     if (dev < 64) set[dev] = true;
   }
   kv8_attn_kernel<KIND, DH><<<ctas, 32, S::BYTES, st>>>(a);
-  if (ctas > 1) {
-    // launched while the first kernel runs; it waits for that one's end itself
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = ctas - 1;
-    cfg.blockDim = 32 * KM_WARPS;
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kv8_attn_merge_kernel<DH>, a) != cudaSuccess) return -3;
-  }
+  const int rc = launch_kv8_merge<DH, KA_ROWS>(a, ctas, st);
+  if (rc != 0) return rc;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
+
+// How a call is cut: the tile (eight rows, or the wide one of kv8_attn_rows.cu), the units of an entry at most,
+// entries of a launch, CTAs of a launch (one for every place on the device, where there is work).
+struct AttnShape {
+  bool wide;
+  int tile, each, ctas;
+  long long units;
+  AttnShape(int n, int rows, int most, int group, int max_pages, int kv_heads, int dh) {
+    if (most > rows) most = rows;                              // a row counts at most once
+    wide = 1ll * most * group > KA_WIDE;
+    tile = wide ? kv8_rows_tile() : KA_ROWS;
+    units = (1ll * most * group + tile - 1) / tile * (max_pages + (wide ? kv8_rows_extra() : KA_EXTRA)) * kv_heads;
+    const long long fit = units > 0 ? 0x7fffffffll / units : 0;
+    each = static_cast<int>(fit < n ? fit : n);
+    if (each > KA_ENTRIES) each = KA_ENTRIES;
+    const int share = wide ? kv8_rows_share() : KA_SHARE;
+    const long long places = static_cast<long long>(wide ? 1 : dh == 64 ? KA_PLACES64 : KA_PLACES) * sm_count();
+    const long long work = (each * units + share - 1) / share;
+    ctas = static_cast<int>(work < places ? work : places);
+  }
+};
 
 }  // namespace cb
 
 using namespace cb;
 
-// Units of an entry at most; entries of a launch; CTAs of a launch: one for every place on the device, where there is work.
-static long long attn_units(int most, int group, int max_pages, int kv_heads) {
-  return (1ll * most * group + KA_ROWS - 1) / KA_ROWS * (max_pages + KA_EXTRA) * kv_heads;
-}
-static int attn_entries(int n, long long units) {
-  const long long fit = 0x7fffffffll / units;
-  return static_cast<int>(fit < n && fit < KA_ENTRIES ? fit : n < KA_ENTRIES ? n : KA_ENTRIES);
-}
-static int attn_ctas(int n, long long units, int dh) {
-  const long long places = static_cast<long long>(dh == 64 ? KA_PLACES64 : KA_PLACES) * sm_count(), work = (n * units + KA_SHARE - 1) / KA_SHARE;
-  return static_cast<int>(work < places ? work : places);
-}
-
 // Bytes of scratch of one call.
 extern "C" int64_t cb_kv8_attn_scratch(int n, int rows, int most, int group, int max_pages, int kv_heads, int dh) {
-  const long long units = attn_units(most < rows ? most : rows, group, max_pages, kv_heads);
-  return attn_ctas(n < KA_ENTRIES ? n : KA_ENTRIES, units, dh) * static_cast<int64_t>(2 * KA_ROWS * (dh + 2) * 4 + sizeof(Kv8Desc)) + 256;
+  const AttnShape s(n, rows, most, group, max_pages, kv_heads, dh);
+  return s.ctas * static_cast<int64_t>(2 * s.tile * (dh + 2) * 4 + sizeof(Kv8Desc)) + 256;
 }
 
 extern "C" int cb_kv8_attn(const void* q, int ldq, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -662,18 +457,17 @@ extern "C" int cb_kv8_attn(const void* q, int ldq, const void* k_cache, const vo
   if (n < 1 || rows < 1 || most < 1 || kv_heads < 1 || heads < 1 || heads % kv_heads != 0) return -1;
   if ((dh != 64 && dh != 128) || (kind != KV8_INT8 && kind != KV8_E4M3)) return -2;
   const int group = heads / kv_heads;
-  if (most > rows) most = rows;                                // a row counts at most once
-  const long long units = attn_units(most, group, max_pages, kv_heads);
-  if (1ll * max_pages * KV8_PAGE > 0x7fffffffll || units > 0x7fffffffll) return -5;
-  const int each = attn_entries(n, units), ctas = attn_ctas(each, units, dh);
+  const AttnShape s(n, rows, most, group, max_pages, kv_heads, dh);
+  if (1ll * max_pages * KV8_PAGE > 0x7fffffffll || s.each < 1) return -5;
+  const int each = s.each, ctas = s.ctas;
   Kv8Attn a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
-  a.ldq = ldq; a.ldo = ldo; a.group = group; a.rows = rows; a.most = most;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.ldq = ldq; a.ldo = ldo; a.group = group; a.rows = rows; a.most = most < rows ? most : rows;
+  a.scale_log2 = scale * KA_LOG2E;
   a.desc = static_cast<Kv8Desc*>(scratch);
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(Kv8Desc) + 255) / 256 * 256);
-  a.part_ml = a.part_o + static_cast<size_t>(ctas) * 2 * KA_ROWS * dh;
+  a.part_ml = a.part_o + static_cast<size_t>(ctas) * 2 * s.tile * dh;
   a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int e0 = 0; e0 < n; e0 += each) {
@@ -685,7 +479,8 @@ extern "C" int cb_kv8_attn(const void* q, int ldq, const void* k_cache, const vo
     a.first = e0;
     a.n = n - e0 < each ? n - e0 : each;
     int rc;
-    if (kind == KV8_INT8) rc = dh == 64 ? launch_attn<KV8_INT8, 64>(a, ctas, st) : launch_attn<KV8_INT8, 128>(a, ctas, st);
+    if (s.wide) rc = launch_kv8_rows(a, kind, dh, ctas, st);
+    else if (kind == KV8_INT8) rc = dh == 64 ? launch_attn<KV8_INT8, 64>(a, ctas, st) : launch_attn<KV8_INT8, 128>(a, ctas, st);
     else rc = dh == 64 ? launch_attn<KV8_E4M3, 64>(a, ctas, st) : launch_attn<KV8_E4M3, 128>(a, ctas, st);
     if (rc != 0) return rc;
   }

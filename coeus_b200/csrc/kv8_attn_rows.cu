@@ -1,0 +1,461 @@
+// Attention over the 8-bit cache for many query rows per sequence (kv8_attn.cu has the mathematics and the
+// kernel for few): tiles of 128 rows (rows and heads that share a key/value head) on the fifth-generation
+// tensor cores, a page of 64 keys at a time.
+//
+//   warps 4 - 7   turn the page's codes into fp16 operands in shared memory (exactly; 128-byte swizzle), the next page
+//                 on its way in registers, and the tile's queries before its first page
+//   warp 8        issues S = Q K^T (one accumulator of two) and O += P V
+//   warps 0 - 3   a row per thread: weights from S, written back as fp16 in tensor memory, where the second product
+//                 reads them; the running maximum, the sum, and at the end the tile's rows
+//
+// The scale 2^ev of a page's values goes into the weights: with z = s + ev (s the score in units of log2) and m a
+// running maximum of z, the weights are P = 2^(z - m), and the denominator sums 2^(e0 - ev) P, e0 the first page's ev:
+// o = 2^e0 sum P code / sum 2^(e0 - ev) P.  So pages of any scales add up in one accumulator.  The maximum is only
+// raised when z exceeds it by more than KB_LAG, and the sums so far are multiplied then.  Bound by the matrix products and the softmax between them: a page of a tile is 2 x 64 x 128 dh
+// multiply-adds and 8192 exponentials.
+#include "kv8_attn.cuh"
+
+namespace cb {
+
+constexpr int KB_ROWS = 128;                      // of a tile
+constexpr int KB_EXTRA = 2;                       // what a tile costs beside its pages, in pages
+constexpr int KB_SHARE = 4;                       // pages a CTA takes at least
+constexpr int KB_THREADS = 288;
+constexpr int KB_STAGES = 3;
+// Weights are held times 2^KB_SHIFT and are at most 2^(KB_SHIFT + KB_LAG) < 65504; fp16 keeps their digits down to 2^-24
+// of the row's largest, and 2^-34 is lost.
+constexpr float KB_SHIFT = 10.f, KB_LAG = 4.f;
+constexpr uint32_t KB_O = 0, KB_S = 128, KB_P = 256, KB_COLS = 512;      // columns of tensor memory
+
+template <int DH>
+struct RowsSmem {
+  static constexpr int PANEL_K = KV8_PAGE * 128;                 // 64 channels of 64 keys, fp16
+  static constexpr int HALVES = DH / 64;
+  static constexpr int V = HALVES * PANEL_K, STAGE = V + DH * 128;      // keys, then values [channel][64 keys]
+  static constexpr int Q = HALVES * KB_ROWS * 128;
+  static constexpr int BYTES = 1024 + Q + KB_STAGES * STAGE + 4 * KB_ROWS * 4 + KB_STAGES * 16 + (KA_ENTRIES + 1) * 4 + 256;
+};
+
+// 16 codes to 16 numbers of fp16 in two vectors.
+template <int KIND>
+__device__ __forceinline__ void half16(const uint4& w, uint4& a, uint4& b) {
+  kv8_half4<KIND>(w.x, a.x, a.y);
+  kv8_half4<KIND>(w.y, a.z, a.w);
+  kv8_half4<KIND>(w.z, b.x, b.y);
+  kv8_half4<KIND>(w.w, b.z, b.w);
+}
+__device__ __forceinline__ constexpr uint32_t idesc_f16(int m, int n) {
+  return umma_idesc_bf16(m, n, 0, 0) & ~((7u << 7) | (7u << 10));        // both operands fp16
+}
+
+template <int KIND, int DH>
+__global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_constant__ Kv8Attn a) {
+  using S = RowsSmem<DH>;
+  constexpr int HALVES = S::HALVES;
+  extern __shared__ __align__(16) unsigned char raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* sq = smem;                                      // [HALVES][128 rows][128 bytes]
+  unsigned char* stage = sq + S::Q;                              // [KB_STAGES][STAGE]
+  float* sf = reinterpret_cast<float*>(stage + KB_STAGES * S::STAGE);      // [4 tiles][128]: score per product
+  float4* meta = reinterpret_cast<float4*>(sf + 4 * KB_ROWS);    // [KB_STAGES]: scales of the page, whether there is one
+  uint64_t* bars = reinterpret_cast<uint64_t*>(meta + KB_STAGES);
+  uint64_t *full = bars, *empty = full + KB_STAGES, *s_full = empty + KB_STAGES, *p_full = s_full + 2, *o_done = p_full + 2;
+  uint64_t *q_full = o_done + 2, *q_free = q_full + 1;
+  int* prefix = reinterpret_cast<int*>(q_free + 1);              // [KA_ENTRIES + 1]
+  __shared__ volatile uint32_t abort_flag;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_units;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkv = a.c.heads;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&tmem_slot), KB_COLS);
+    tmem_relinquish();
+  } else if (warp == 0) {
+    const int n = kv8_plan(a, KB_ROWS, KB_EXTRA, prefix, lane);
+    if (lane == 0) s_units = n;
+  }
+  if (tid == 64) {
+    abort_flag = 0u;
+    for (int i = 0; i < KB_STAGES; ++i) {
+      mbar_init(smem_u32(full + i), 128);
+      mbar_init(smem_u32(empty + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(s_full + i), 1);
+      mbar_init(smem_u32(p_full + i), 128);
+      mbar_init(smem_u32(o_done + i), 1);
+    }
+    mbar_init(smem_u32(q_full), 128);
+    mbar_init(smem_u32(q_free), 1);
+    mbar_fence_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int units = s_units, share = max((units - 1) / static_cast<int>(gridDim.x) + 1, KB_SHARE);
+  const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(share) * blockIdx.x));
+  const int u1 = min(units - u0, share) + u0;
+  if (tid == 0) kv8_describe(a, KB_ROWS, KB_EXTRA, prefix, u0, u1 - u0, share, units);
+  kv8_zero_rows<DH>(a, tid, KB_THREADS);
+
+  // A tile's pages here: p0 .. p1 - 1 (none for its extra units, or if no row of it sees that far).
+  struct Piece {
+    Kv8Where w;
+    int p0, p1;
+    bool any, whole, begins;           // there are pages at all; all of the tile is here; it is the CTA's first tile
+  };
+  auto piece_at = [&](int u) {
+    Piece t;
+    t.w = kv8_locate(a, KB_ROWS, KB_EXTRA, prefix, u);
+    t.p0 = u - t.w.lo;
+    const int end = min(t.w.pages, u1 - t.w.lo), last = min(t.w.x.rows - 1, (t.w.tile * KB_ROWS + KB_ROWS - 1) / a.group);
+    const int all_seen = t.w.x.ctx - t.w.x.rows + last + 1;
+    t.any = t.p0 < end;
+    t.p1 = min(end, (max(all_seen, 0) + KV8_PAGE - 1) / KV8_PAGE);
+    t.whole = t.w.lo >= u0 && t.w.lo + t.w.pages <= u1;
+    t.begins = t.w.lo <= u0;
+    return t;
+  };
+  auto next_tile = [&](const Piece& t) { return t.w.lo + t.w.pages + KB_EXTRA; };
+  bool dead = false;
+  auto wait = [&](uint64_t* bar, int n) {                        // the n-th phase (from 0)
+    if (dead) return;
+    if (!wait_phase(bar, n & 1, &abort_flag)) {
+      dead = true;
+      record_status(a.status, ST_WAIT_TIMEOUT, blockIdx.x);
+    }
+  };
+
+  if (warp >= 4 && warp < 8) {
+    // ---- operands
+    const int t0 = tid - 128;
+    int gi = 0, tiles = 0;                                       // pages and tiles so far
+    constexpr int VECS = DH / 32;                                // 16-byte vectors of codes of a thread, keys and values each
+    for (int u = u0; u < u1;) {
+      const Piece t = piece_at(u);
+      u = next_tile(t);
+      if (!t.any || t.p0 >= t.p1) continue;
+      const int* table = a.c.page_table + static_cast<size_t>(t.w.e) * a.c.max_pages;
+      auto page_of = [&](int p) { return p < t.p1 ? __ldg(table + p) : 0; };
+      uint4 kc[VECS], vc[VECS];
+      float ks = 0.f, vs = 0.f;
+      int ok = 0;
+      auto fetch = [&](int page) {                               // the page's codes are on their way
+        ok = page >= 0 && page < a.c.num_pages;
+        if (!ok) {
+          if (t0 == 0) record_status(a.status, ST_BOUNDS, t.w.e);
+          page = 0;
+        }
+        const size_t cell = static_cast<size_t>(page) * nkv + t.w.hk;
+        const uint4* k = reinterpret_cast<const uint4*>(a.c.k + cell * (KV8_PAGE * DH)) + t0;
+        const uint4* v = reinterpret_cast<const uint4*>(a.c.v + cell * (KV8_PAGE * DH)) + t0;
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          kc[i] = __ldg(k + 128 * i);
+          vc[i] = __ldg(v + 128 * i);
+        }
+        ks = __ldg(a.c.k_scale + cell);
+        vs = __ldg(a.c.v_scale + cell);
+      };
+      fetch(page_of(t.p0));
+      int page = page_of(t.p0 + 1);
+      // the tile's queries: a row per thread, divided by the binade of its largest number
+      if (tiles > 0) wait(q_free, tiles - 1);
+      {
+        const int r = t.w.tile * KB_ROWS + t0;
+        const bool in = r < t.w.x.rows * a.group;
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + (in ? static_cast<size_t>(t.w.x.first + r / a.group) * a.ldq + (t.w.hk * a.group + r % a.group) * DH : 0));
+        float top = 0.f;
+        if (in)
+#pragma unroll 4
+          for (int i = 0; i < DH / 8; ++i) {
+            const uint4 x = __ldg(src + i);
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 b = unpack_bf16x2(v[j]);
+              top = fmaxf(top, fmaxf(fabsf(b.x), fabsf(b.y)));
+            }
+          }
+        const int k = top > 0.f && top < INFINITY ? max(min((__float_as_int(top) >> 23) - 127, 126), -126) : 0;
+        const float down = pow2(-k);
+        sf[(tiles & 3) * KB_ROWS + t0] = pow2(k) * a.scale_log2;
+#pragma unroll 4
+        for (int i = 0; i < DH / 8; ++i) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (in) {
+            x = __ldg(src + i);
+            uint32_t* v = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 b = unpack_bf16x2(v[j]);
+              v[j] = half2_bits(b.x * down, b.y * down);
+            }
+          }
+          *reinterpret_cast<uint4*>(sq + (i / 8 * KB_ROWS + t0) * 128 + ((i & 7) ^ (t0 & 7)) * 16) = x;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(q_full));
+      ++tiles;
+      const int last = min(t.w.x.rows - 1, (t.w.tile * KB_ROWS + KB_ROWS - 1) / a.group);
+      const int all_seen = t.w.x.ctx - t.w.x.rows + last + 1;
+      for (int p = t.p0; p < t.p1; ++p, ++gi) {
+        const int st = gi % KB_STAGES;
+        if (gi >= KB_STAGES) wait(empty + st, gi / KB_STAGES - 1);
+        unsigned char* kd = stage + st * S::STAGE;
+        unsigned char* vd = kd + S::V;
+        const int left = all_seen - p * KV8_PAGE;                // tokens of the page that any row sees
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          const int x = t0 + 128 * i, row = x >> 2, c = x & 3;   // keys: row of every half in turn
+          uint4 lo, hi;
+          half16<KIND>(kc[i], lo, hi);
+          unsigned char* d = kd + row * 128;
+          *reinterpret_cast<uint4*>(d + ((2 * c) ^ (row & 7)) * 16) = lo;
+          *reinterpret_cast<uint4*>(d + ((2 * c + 1) ^ (row & 7)) * 16) = hi;
+          if (left < KV8_PAGE) {
+            // codes of values that no row sees may be anything (not a number even): zero times them is not zero
+            uint32_t* w = reinterpret_cast<uint32_t*>(&vc[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int over = left - 16 * c - 4 * j;
+              w[j] &= over >= 4 ? 0xffffffffu : over <= 0 ? 0u : (1u << (8 * over)) - 1u;
+            }
+          }
+          half16<KIND>(vc[i], lo, hi);
+          d = vd + row * 128;
+          *reinterpret_cast<uint4*>(d + ((2 * c) ^ (row & 7)) * 16) = lo;
+          *reinterpret_cast<uint4*>(d + ((2 * c + 1) ^ (row & 7)) * 16) = hi;
+        }
+        if (t0 == 0) meta[st] = make_float4(ks, vs, ok ? 1.f : 0.f, 0.f);
+        if (p + 1 < t.p1) {
+          fetch(page);
+          page = page_of(p + 2);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(full + st));
+      }
+    }
+  } else if (warp == 8) {
+    // ---- the products, by one thread
+    if (elect_one()) {
+      constexpr uint32_t id_s = idesc_f16(KB_ROWS, KV8_PAGE), id_o = idesc_f16(KB_ROWS, DH);
+      int gi = 0, tiles = 0;
+      auto scores = [&](int i) {
+        const int st = i % KB_STAGES;
+        wait(full + st, i / KB_STAGES);
+        if (dead) return;
+        tc_fence_after();
+        const uint32_t kd = smem_u32(stage + st * S::STAGE);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16_ss(tmem + KB_S + (i & 1) * KV8_PAGE, umma_desc_sw128(smem_u32(sq) + h * KB_ROWS * 128 + k * 32, 16, 1024),
+                         umma_desc_sw128(kd + h * S::PANEL_K + k * 32, 16, 1024), id_s, h + k > 0 ? 1u : 0u);
+        umma_commit(smem_u32(s_full + (i & 1)));
+      };
+      for (int u = u0; u < u1;) {
+        const Piece t = piece_at(u);
+        u = next_tile(t);
+        if (!t.any || t.p0 >= t.p1) continue;
+        const int n = t.p1 - t.p0;
+        wait(q_full, tiles++);
+        scores(gi);
+        if (n == 1) umma_commit(smem_u32(q_free));
+        for (int i = 0; i < n; ++i, ++gi) {
+          if (i + 1 < n) scores(gi + 1);
+          if (i + 2 == n) umma_commit(smem_u32(q_free));
+          wait(p_full + (gi & 1), gi >> 1);
+          if (dead) break;
+          tc_fence_after();
+          const int st = gi % KB_STAGES;
+          const uint32_t vd = smem_u32(stage + st * S::STAGE + S::V);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16_ts(tmem + KB_O, tmem + KB_P + (gi & 1) * 32 + k * 8, umma_desc_sw128(vd + k * 32, 16, 1024), id_o, i + k > 0 ? 1u : 0u);
+          umma_commit(smem_u32(empty + st));
+          umma_commit(smem_u32(o_done + (gi & 1)));
+        }
+        if (dead) break;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- weights: a row per thread
+    const uint32_t mine = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    int gi = 0, tiles = 0;
+    for (int u = u0; u < u1;) {
+      const Piece t = piece_at(u);
+      u = next_tile(t);
+      if (!t.any) continue;
+      const int rows = t.w.x.rows, ctx = t.w.x.ctx, total = rows * a.group, rr = t.w.tile * KB_ROWS + tid;
+      const int seen = ctx - rows + min(rr, total - 1) / a.group + 1;
+      const int least_seen = ctx - rows + t.w.tile * KB_ROWS / a.group + 1;
+      float m = -INFINITY, l = 0.f, f = 0.f;
+      int e0 = 0, e_top = -1000;                                 // the first page's scale, the largest so far
+      for (int p = t.p0; p < t.p1; ++p, ++gi) {
+        const int st = gi % KB_STAGES, base = p * KV8_PAGE;
+        wait(full + st, gi / KB_STAGES);
+        wait(s_full + (gi & 1), gi >> 1);
+        if (dead) break;
+        tc_fence_after();
+        if (p == t.p0) f = sf[(tiles & 3) * KB_ROWS + tid];
+        const float4 mt = meta[st];
+        float s[64];
+        uint32_t* bits = reinterpret_cast<uint32_t*>(s);
+        tmem_ld_32x32b_x32(mine + KB_S + (gi & 1) * KV8_PAGE, bits);
+        tmem_ld_32x32b_x32(mine + KB_S + (gi & 1) * KV8_PAGE + 32, bits + 32);
+        tmem_ld_wait();
+        // A page without values (the smallest scale there is) has weights for the denominator only, under whatever scale;
+        // one whose values are next to nothing against another's counts as if they were 2^-40 of these.
+        const bool fine = mt.y == mt.y, none = fine && mt.y <= 1.17549435e-38f;
+        int ev = fine ? (__float_as_int(mt.y) >> 23) - 127 : 0;
+        if (fine && !none) {
+          e_top = max(e_top, ev);
+          ev = max(ev, e_top - 40);
+        } else {
+          ev = e_top > -1000 ? e_top : 0;
+        }
+        if (p == t.p0) e0 = ev;
+        const float fk = f * mt.x, ef = fine ? static_cast<float>(ev) : mt.y;
+        const bool whole = base + KV8_PAGE <= least_seen && mt.z != 0.f;
+        const int n_seen = mt.z != 0.f ? seen - base : 0;        // keys of the page that the row sees
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= n_seen) s[i] = -INFINITY;
+        }
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < 64; i += 4)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[i + j]);
+        const float z = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fk, ef);       // NaN: no maximum
+        const bool raise = z > m + KB_LAG || (m == -INFINITY && z > -INFINITY);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = raise ? z : m;
+          const float c = mn == m ? 1.f : fast_exp2(m - mn);
+          m = mn;
+          l *= c;
+          if (p > t.p0) {                                        // the sums so far: the last product is over
+            wait(o_done + ((gi - 1) & 1), (gi - 1) >> 1);
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < DH; i += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(mine + KB_O + i, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
+              tmem_st_32x32b_x16(mine + KB_O + i, o);
+              tmem_st_32x32b_x16(mine + KB_O + i + 16, o + 16);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float sub = KB_SHIFT + ef - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] = fast_exp2(fmaf(s[i], fk, sub));
+        if (!whole) {                                            // whatever the scales are
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= n_seen) s[i] = 0.f;
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = none ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 64; i += 4)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[j] += s[i + j];
+        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(max(min(e0 - ev, 100), -126)), l);
+        if (gi >= 2) wait(o_done + (gi & 1), (gi >> 1) - 1);     // the product that read these columns is over
+        tmem_st_32x32b_x16(mine + KB_P + (gi & 1) * 32, w);
+        tmem_st_32x32b_x16(mine + KB_P + (gi & 1) * 32 + 16, w + 16);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(p_full + (gi & 1)));
+      }
+      if (dead) break;
+      // ---- the tile's rows, or this CTA's part of them
+      const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (t.begins ? 0 : 1);
+      const bool summed = t.p0 < t.p1;
+      if (summed) {
+        ++tiles;
+        wait(o_done + ((gi - 1) & 1), (gi - 1) >> 1);
+        if (dead) break;
+        tc_fence_after();
+      }
+      const float up = pow2(max(e0, -126)), inv = seen > 0 && summed ? up / l : 0.f;
+      __nv_bfloat16* dst = a.out + static_cast<size_t>(t.w.x.first + rr / a.group) * a.ldo + (t.w.hk * a.group + rr % a.group) * DH;
+#pragma unroll
+      for (int i = 0; i < DH; i += 32) {
+        uint32_t o[32];
+        if (summed) {
+          tmem_ld_32x32b_x32(mine + KB_O + i, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+        if (rr < total) {
+          if (t.whole) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              float v[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) v[x] = seen > 0 ? __uint_as_float(o[j + x]) * inv : 0.f;
+              store8(dst + i + j, v);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<uint4*>(a.part_o + (slot * KB_ROWS + tid) * DH + i + j) = 
+                  make_uint4(__float_as_uint(__uint_as_float(o[j]) * up), __float_as_uint(__uint_as_float(o[j + 1]) * up),
+                             __float_as_uint(__uint_as_float(o[j + 2]) * up), __float_as_uint(__uint_as_float(o[j + 3]) * up));
+          }
+        }
+      }
+      if (!t.whole && rr < total) *reinterpret_cast<float2*>(a.part_ml + (slot * KB_ROWS + tid) * 2) = make_float2(m - static_cast<float>(e0), l);
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, KB_COLS);
+  }
+}
+
+template <int KIND, int DH>
+static int launch_rows(const Kv8Attn& a, int ctas, cudaStream_t st) {
+  using S = RowsSmem<DH>;
+  static bool set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -4;
+  // more than half of an SM's shared memory: one CTA, which takes all of its tensor memory
+  const int bytes = S::BYTES > 120 * 1024 ? S::BYTES : 120 * 1024;
+  if (dev >= 64 || !set[dev]) {
+    if (cudaFuncSetAttribute(kv8_rows_kernel<KIND, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return -4;
+    if (dev < 64) set[dev] = true;
+  }
+  kv8_rows_kernel<KIND, DH><<<ctas, KB_THREADS, bytes, st>>>(a);
+  const int rc = launch_kv8_merge<DH, KB_ROWS>(a, ctas, st);
+  if (rc != 0) return rc;
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+int launch_kv8_rows(const Kv8Attn& a, int kind, int dh, int ctas, cudaStream_t st) {
+  if (kind == KV8_INT8) return dh == 64 ? launch_rows<KV8_INT8, 64>(a, ctas, st) : launch_rows<KV8_INT8, 128>(a, ctas, st);
+  return dh == 64 ? launch_rows<KV8_E4M3, 64>(a, ctas, st) : launch_rows<KV8_E4M3, 128>(a, ctas, st);
+}
+int kv8_rows_tile() { return KB_ROWS; }
+int kv8_rows_share() { return KB_SHARE; }
+int kv8_rows_extra() { return KB_EXTRA; }
+
+}  // namespace cb

@@ -4,7 +4,8 @@
 //
 //   warps 4 - 7   turn the page's codes into fp16 operands in shared memory (exactly; 128-byte swizzle), the next page
 //                 on its way in registers, and the tile's queries before its first page
-//   warp 8        issues S = Q K^T (one accumulator of two) and O += P V
+//   warp 8        issues S = Q K^T (one accumulator of two), warp 9 O += P V: one thread for both needed about 1500 cycles
+//                 a page to issue them, more than they take
 //   warps 0 - 3   a row per thread: weights from S, written back as fp16 in tensor memory, where the second product
 //                 reads them; the running maximum, the sum, and at the end the tile's rows
 //
@@ -20,7 +21,7 @@ namespace cb {
 constexpr int KB_ROWS = 128;                      // of a tile
 constexpr int KB_EXTRA = 2;                       // what a tile costs beside its pages, in pages
 constexpr int KB_SHARE = 4;                       // pages a CTA takes at least
-constexpr int KB_THREADS = 288;
+constexpr int KB_THREADS = 320;
 constexpr int KB_STAGES = 3;
 // Weights are held times 2^KB_SHIFT and are at most 2^(KB_SHIFT + KB_LAG) < 65504; fp16 keeps their digits down to 2^-24
 // of the row's largest, and 2^-34 is lost.
@@ -140,25 +141,28 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
       auto page_of = [&](int p) { return p < t.p1 ? __ldg(table + p) : 0; };
       uint4 kc[VECS], vc[VECS];
       float ks = 0.f, vs = 0.f;
-      int ok = 0;
-      auto fetch = [&](int page) {                               // the page's codes are on their way
-        ok = page >= 0 && page < a.c.num_pages;
-        if (!ok) {
+      const uint4 *kn, *vn;                                      // the next page's codes
+      size_t cell_n = 0;
+      int ok_n = 0;
+      auto aim = [&](int page) {
+        ok_n = page >= 0 && page < a.c.num_pages;
+        if (!ok_n) {
           if (t0 == 0) record_status(a.status, ST_BOUNDS, t.w.e);
           page = 0;
         }
-        const size_t cell = static_cast<size_t>(page) * nkv + t.w.hk;
-        const uint4* k = reinterpret_cast<const uint4*>(a.c.k + cell * (KV8_PAGE * DH)) + t0;
-        const uint4* v = reinterpret_cast<const uint4*>(a.c.v + cell * (KV8_PAGE * DH)) + t0;
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) {
-          kc[i] = __ldg(k + 128 * i);
-          vc[i] = __ldg(v + 128 * i);
-        }
-        ks = __ldg(a.c.k_scale + cell);
-        vs = __ldg(a.c.v_scale + cell);
+        cell_n = static_cast<size_t>(page) * nkv + t.w.hk;
+        kn = reinterpret_cast<const uint4*>(a.c.k + cell_n * (KV8_PAGE * DH)) + t0;
+        vn = reinterpret_cast<const uint4*>(a.c.v + cell_n * (KV8_PAGE * DH)) + t0;
       };
-      fetch(page_of(t.p0));
+      aim(page_of(t.p0));
+      int ok = ok_n;
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        kc[i] = __ldg(kn + 128 * i);
+        vc[i] = __ldg(vn + 128 * i);
+      }
+      ks = __ldg(a.c.k_scale + cell_n);
+      vs = __ldg(a.c.v_scale + cell_n);
       int page = page_of(t.p0 + 1);
       // the tile's queries: a row per thread, divided by the binade of its largest number
       if (tiles > 0) wait(q_free, tiles - 1);
@@ -205,81 +209,99 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
         const int st = gi % KB_STAGES;
         if (gi >= KB_STAGES) wait(empty + st, gi / KB_STAGES - 1);
         unsigned char* kd = stage + st * S::STAGE;
-        unsigned char* vd = kd + S::V;
         const int left = all_seen - p * KV8_PAGE;                // tokens of the page that any row sees
+        if (t0 == 0) meta[st] = make_float4(ks, vs, ok ? 1.f : 0.f, 0.f);
+        const bool more = p + 1 < t.p1;
+        if (more) {
+          aim(page);
+          page = page_of(p + 2);
+          ok = ok_n;
+          ks = __ldg(a.c.k_scale + cell_n);
+          vs = __ldg(a.c.v_scale + cell_n);
+        }
+        if (left < KV8_PAGE) {
+          // codes of values that no row sees may be anything (not a number even): zero times them is not zero
 #pragma unroll
-        for (int i = 0; i < VECS; ++i) {
-          const int x = t0 + 128 * i, row = x >> 2, c = x & 3;   // keys: row of every half in turn
-          uint4 lo, hi;
-          half16<KIND>(kc[i], lo, hi);
-          unsigned char* d = kd + row * 128;
-          *reinterpret_cast<uint4*>(d + ((2 * c) ^ (row & 7)) * 16) = lo;
-          *reinterpret_cast<uint4*>(d + ((2 * c + 1) ^ (row & 7)) * 16) = hi;
-          if (left < KV8_PAGE) {
-            // codes of values that no row sees may be anything (not a number even): zero times them is not zero
+          for (int i = 0; i < VECS; ++i) {
             uint32_t* w = reinterpret_cast<uint32_t*>(&vc[i]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int over = left - 16 * c - 4 * j;
+              const int over = left - 16 * (t0 & 3) - 4 * j;
               w[j] &= over >= 4 ? 0xffffffffu : over <= 0 ? 0u : (1u << (8 * over)) - 1u;
             }
           }
-          half16<KIND>(vc[i], lo, hi);
-          d = vd + row * 128;
-          *reinterpret_cast<uint4*>(d + ((2 * c) ^ (row & 7)) * 16) = lo;
-          *reinterpret_cast<uint4*>(d + ((2 * c + 1) ^ (row & 7)) * 16) = hi;
         }
-        if (t0 == 0) meta[st] = make_float4(ks, vs, ok ? 1.f : 0.f, 0.f);
-        if (p + 1 < t.p1) {
-          fetch(page);
-          page = page_of(p + 2);
+        // row x >> 2 of the operand, 16 codes x & 3 of it; the next page's are asked for as soon as these are used
+        unsigned char* const d0 = kd + (t0 >> 2) * 128;
+        const int c0 = ((2 * (t0 & 3)) ^ (t0 >> 2 & 7)) * 16, c1 = c0 ^ 16;    // 32 rows on the swizzle is the same
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          uint4 lo, hi;
+          half16<KIND>(kc[i], lo, hi);
+          if (more) kc[i] = __ldg(kn + 128 * i);
+          *reinterpret_cast<uint4*>(d0 + i * 4096 + c0) = lo;
+          *reinterpret_cast<uint4*>(d0 + i * 4096 + c1) = hi;
+          half16<KIND>(vc[i], lo, hi);
+          if (more) vc[i] = __ldg(vn + 128 * i);
+          *reinterpret_cast<uint4*>(d0 + S::V + i * 4096 + c0) = lo;
+          *reinterpret_cast<uint4*>(d0 + S::V + i * 4096 + c1) = hi;
         }
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(full + st));
       }
     }
   } else if (warp == 8) {
-    // ---- the products, by one thread
+    // ---- scores, issued by one thread
     if (elect_one()) {
-      constexpr uint32_t id_s = idesc_f16(KB_ROWS, KV8_PAGE), id_o = idesc_f16(KB_ROWS, DH);
+      constexpr uint32_t id_s = idesc_f16(KB_ROWS, KV8_PAGE);
+      const uint64_t dq = umma_desc_sw128(smem_u32(sq), 16, 1024), dk = umma_desc_sw128(smem_u32(stage), 16, 1024);
       int gi = 0, tiles = 0;
-      auto scores = [&](int i) {
-        const int st = i % KB_STAGES;
-        wait(full + st, i / KB_STAGES);
-        if (dead) return;
-        tc_fence_after();
-        const uint32_t kd = smem_u32(stage + st * S::STAGE);
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ss(tmem + KB_S + (i & 1) * KV8_PAGE, umma_desc_sw128(smem_u32(sq) + h * KB_ROWS * 128 + k * 32, 16, 1024),
-                         umma_desc_sw128(kd + h * S::PANEL_K + k * 32, 16, 1024), id_s, h + k > 0 ? 1u : 0u);
-        umma_commit(smem_u32(s_full + (i & 1)));
-      };
-      for (int u = u0; u < u1;) {
+      for (int u = u0; u < u1 && !dead;) {
         const Piece t = piece_at(u);
         u = next_tile(t);
         if (!t.any || t.p0 >= t.p1) continue;
-        const int n = t.p1 - t.p0;
         wait(q_full, tiles++);
-        scores(gi);
-        if (n == 1) umma_commit(smem_u32(q_free));
-        for (int i = 0; i < n; ++i, ++gi) {
-          if (i + 1 < n) scores(gi + 1);
-          if (i + 2 == n) umma_commit(smem_u32(q_free));
+        for (int n = t.p1 - t.p0; n > 0; --n, ++gi) {
+          const int st = gi % KB_STAGES;
+          wait(full + st, gi / KB_STAGES);
+          if (gi >= 2) wait(p_full + (gi & 1), (gi >> 1) - 1);   // the scores that were here have been read
+          if (dead) break;
+          tc_fence_after();
+          const uint64_t dks = dk + st * (S::STAGE >> 4);
+          const uint32_t d = tmem + KB_S + (gi & 1) * KV8_PAGE;
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_ss(d, dq + ((h * KB_ROWS * 128 + k * 32) >> 4), dks + ((h * S::PANEL_K + k * 32) >> 4), id_s, h + k > 0 ? 1u : 0u);
+          umma_commit(smem_u32(s_full + (gi & 1)));
+        }
+        umma_commit(smem_u32(q_free));
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---- weighted values
+    if (elect_one()) {
+      constexpr uint32_t id_o = idesc_f16(KB_ROWS, DH);
+      const uint64_t dv = umma_desc_sw128(smem_u32(stage + S::V), 16, 1024);
+      int gi = 0;
+      for (int u = u0; u < u1 && !dead;) {
+        const Piece t = piece_at(u);
+        u = next_tile(t);
+        if (!t.any) continue;
+        for (int p = t.p0; p < t.p1; ++p, ++gi) {
           wait(p_full + (gi & 1), gi >> 1);
           if (dead) break;
           tc_fence_after();
           const int st = gi % KB_STAGES;
-          const uint32_t vd = smem_u32(stage + st * S::STAGE + S::V);
+          const uint64_t dvs = dv + st * (S::STAGE >> 4);
+          const uint32_t pa = tmem + KB_P + (gi & 1) * 32;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ts(tmem + KB_O, tmem + KB_P + (gi & 1) * 32 + k * 8, umma_desc_sw128(vd + k * 32, 16, 1024), id_o, i + k > 0 ? 1u : 0u);
-          umma_commit(smem_u32(empty + st));
+          for (int k = 0; k < 4; ++k) umma_bf16_ts(tmem + KB_O, pa + k * 8, dvs + ((k * 32) >> 4), id_o, k > 0 || p > t.p0 ? 1u : 0u);
           umma_commit(smem_u32(o_done + (gi & 1)));
+          umma_commit(smem_u32(empty + st));
         }
-        if (dead) break;
       }
     }
     __syncwarp();
@@ -330,9 +352,11 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < 64; i += 4)
+        for (int i = 4; i < 60; i += 8)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[i + j]);
+          for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[60 + j]);
         const float z = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fk, ef);       // NaN: no maximum
         const bool raise = z > m + KB_LAG || (m == -INFINITY && z > -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
@@ -358,7 +382,11 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
         }
         const float sub = KB_SHIFT + ef - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] = fast_exp2(fmaf(s[i], fk, sub));
+        for (int i = 0; i < 64; i += 2) {
+          fma2(s[i], s[i + 1], s[i], s[i + 1], fk, fk, sub, sub);
+          s[i] = fast_exp2(s[i]);
+          s[i + 1] = fast_exp2(s[i + 1]);
+        }
         if (!whole) {                                            // whatever the scales are
 #pragma unroll
           for (int i = 0; i < 64; ++i)
@@ -369,9 +397,10 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = none ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
 #pragma unroll
-        for (int i = 0; i < 64; i += 4)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sum[j] += s[i + j];
+        for (int i = 0; i < 64; i += 4) {
+          add2(sum[0], sum[1], sum[0], sum[1], s[i], s[i + 1]);
+          add2(sum[2], sum[3], sum[2], sum[3], s[i + 2], s[i + 3]);
+        }
         l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(max(min(e0 - ev, 100), -126)), l);
         if (gi >= 2) wait(o_done + (gi & 1), (gi >> 1) - 1);     // the product that read these columns is over
         tmem_st_32x32b_x16(mine + KB_P + (gi & 1) * 32, w);

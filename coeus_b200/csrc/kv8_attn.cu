@@ -54,6 +54,7 @@ int launch_kv8_rows(const Kv8Attn& a, int kind, int dh, int ctas, cudaStream_t s
 int kv8_rows_tile();
 int kv8_rows_share();
 int kv8_rows_extra();
+int kv8_rows_places();
 
 // A unit as it is planned: a page of a tile, and the tile's share of the CTA's units (counted from 0).
 struct Kv8Unit {
@@ -434,7 +435,7 @@ struct AttnShape {
     each = static_cast<int>(fit < n ? fit : n);
     if (each > KA_ENTRIES) each = KA_ENTRIES;
     const int share = wide ? kv8_rows_share() : KA_SHARE;
-    const long long places = static_cast<long long>(wide ? 1 : dh == 64 ? KA_PLACES64 : KA_PLACES) * sm_count();
+    const long long places = static_cast<long long>(wide ? kv8_rows_places() : dh == 64 ? KA_PLACES64 : KA_PLACES) * sm_count();
     const long long work = (each * units + share - 1) / share;
     ctas = static_cast<int>(work < places ? work : places);
   }

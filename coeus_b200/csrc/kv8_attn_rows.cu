@@ -22,11 +22,12 @@ constexpr int KB_ROWS = 128;                      // of a tile
 constexpr int KB_EXTRA = 2;                       // what a tile costs beside its pages, in pages
 constexpr int KB_SHARE = 4;                       // pages a CTA takes at least
 constexpr int KB_THREADS = 320;
-constexpr int KB_STAGES = 3;
+constexpr int KB_STAGES = 2;
+constexpr int KB_PLACES = 2;                      // CTAs that share an SM: the waits of one are the other's time
 // Weights are held times 2^KB_SHIFT and are at most 2^(KB_SHIFT + KB_LAG) < 65504; fp16 keeps their digits down to 2^-24
 // of the row's largest, and 2^-34 is lost.
 constexpr float KB_SHIFT = 10.f, KB_LAG = 4.f;
-constexpr uint32_t KB_O = 0, KB_S = 128, KB_P = 256, KB_COLS = 512;      // columns of tensor memory
+constexpr uint32_t KB_O = 0, KB_S = 128, KB_COLS = 256;                  // columns of tensor memory; weights lie on their scores
 
 template <int DH>
 struct RowsSmem {
@@ -50,7 +51,7 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(int m, int n) {
 }
 
 template <int KIND, int DH>
-__global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_constant__ Kv8Attn a) {
+__global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const __grid_constant__ Kv8Attn a) {
   using S = RowsSmem<DH>;
   constexpr int HALVES = S::HALVES;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
         for (int n = t.p1 - t.p0; n > 0; --n, ++gi) {
           const int st = gi % KB_STAGES;
           wait(full + st, gi / KB_STAGES);
-          if (gi >= 2) wait(p_full + (gi & 1), (gi >> 1) - 1);   // the scores that were here have been read
+          if (gi >= 2) wait(o_done + (gi & 1), (gi >> 1) - 1);   // the weights that were here have been used
           if (dead) break;
           tc_fence_after();
           const uint64_t dks = dk + st * (S::STAGE >> 4);
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
           tc_fence_after();
           const int st = gi % KB_STAGES;
           const uint64_t dvs = dv + st * (S::STAGE >> 4);
-          const uint32_t pa = tmem + KB_P + (gi & 1) * 32;
+          const uint32_t pa = tmem + KB_S + (gi & 1) * KV8_PAGE;
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_bf16_ts(tmem + KB_O, pa + k * 8, dvs + ((k * 32) >> 4), id_o, k > 0 || p > t.p0 ? 1u : 0u);
           umma_commit(smem_u32(o_done + (gi & 1)));
@@ -326,11 +327,7 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
         tc_fence_after();
         if (p == t.p0) f = sf[(tiles & 3) * KB_ROWS + tid];
         const float4 mt = meta[st];
-        float s[64];
-        uint32_t* bits = reinterpret_cast<uint32_t*>(s);
-        tmem_ld_32x32b_x32(mine + KB_S + (gi & 1) * KV8_PAGE, bits);
-        tmem_ld_32x32b_x32(mine + KB_S + (gi & 1) * KV8_PAGE + 32, bits + 32);
-        tmem_ld_wait();
+        const uint32_t sa = mine + KB_S + (gi & 1) * KV8_PAGE;
         // A page without values (the smallest scale there is) has weights for the denominator only, under whatever scale;
         // one whose values are next to nothing against another's counts as if they were 2^-40 of these.
         const bool fine = mt.y == mt.y, none = fine && mt.y <= 1.17549435e-38f;
@@ -345,18 +342,23 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
         const float fk = f * mt.x, ef = fine ? static_cast<float>(ev) : mt.y;
         const bool whole = base + KV8_PAGE <= least_seen && mt.z != 0.f;
         const int n_seen = mt.z != 0.f ? seen - base : 0;        // keys of the page that the row sees
-        if (!whole) {
+        // The row's scores twice, 32 at a time (two CTAs leave a thread 96 registers): for the maximum, then for the weights.
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= n_seen) s[i] = -INFINITY;
+        for (int h = 0; h < 2; ++h) {
+          float s[32];
+          tmem_ld_32x32b_x32(sa + 32 * h, reinterpret_cast<uint32_t*>(s));
+          tmem_ld_wait();
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * h + i >= n_seen) s[i] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
         }
-        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < 60; i += 8)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[60 + j]);
         const float z = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fk, ef);       // NaN: no maximum
         const bool raise = z > m + KB_LAG || (m == -INFINITY && z > -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
@@ -381,30 +383,34 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
           }
         }
         const float sub = KB_SHIFT + ef - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          fma2(s[i], s[i + 1], s[i], s[i + 1], fk, fk, sub, sub);
-          s[i] = fast_exp2(s[i]);
-          s[i + 1] = fast_exp2(s[i + 1]);
-        }
-        if (!whole) {                                            // whatever the scales are
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= n_seen) s[i] = 0.f;
-        }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) w[i] = none ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
+        for (int h = 0; h < 2; ++h) {
+          float s[32];
+          tmem_ld_32x32b_x32(sa + 32 * h, reinterpret_cast<uint32_t*>(s));
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          add2(sum[0], sum[1], sum[0], sum[1], s[i], s[i + 1]);
-          add2(sum[2], sum[3], sum[2], sum[3], s[i + 2], s[i + 3]);
+          for (int i = 0; i < 32; i += 2) {
+            fma2(s[i], s[i + 1], s[i], s[i + 1], fk, fk, sub, sub);
+            s[i] = fast_exp2(s[i]);
+            s[i + 1] = fast_exp2(s[i + 1]);
+          }
+          if (!whole) {                                          // whatever the scales are
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * h + i >= n_seen) s[i] = 0.f;
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            add2(sum[0], sum[1], sum[0], sum[1], s[i], s[i + 1]);
+            add2(sum[2], sum[3], sum[2], sum[3], s[i + 2], s[i + 3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = none ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
+          tmem_st_32x32b_x16(sa + 16 * h, w);                    // on scores that have been read
         }
         l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(max(min(e0 - ev, 100), -126)), l);
-        if (gi >= 2) wait(o_done + (gi & 1), (gi >> 1) - 1);     // the product that read these columns is over
-        tmem_st_32x32b_x16(mine + KB_P + (gi & 1) * 32, w);
-        tmem_st_32x32b_x16(mine + KB_P + (gi & 1) * 32 + 16, w + 16);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(p_full + (gi & 1)));
@@ -461,14 +467,16 @@ __global__ void __launch_bounds__(KB_THREADS, 1) kv8_rows_kernel(const __grid_co
   }
 }
 
+static_assert(RowsSmem<128>::BYTES <= 113 * 1024 && KB_PLACES * KB_COLS <= 512, "two CTAs per SM");
+
 template <int KIND, int DH>
 static int launch_rows(const Kv8Attn& a, int ctas, cudaStream_t st) {
   using S = RowsSmem<DH>;
   static bool set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -4;
-  // more than half of an SM's shared memory: one CTA, which takes all of its tensor memory
-  const int bytes = S::BYTES > 120 * 1024 ? S::BYTES : 120 * 1024;
+  // at least a third of an SM's shared memory, so that no more CTAs share it than its tensor memory has columns for
+  const int bytes = S::BYTES > 80 * 1024 ? S::BYTES : 80 * 1024;
   if (dev >= 64 || !set[dev]) {
     if (cudaFuncSetAttribute(kv8_rows_kernel<KIND, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return -4;
@@ -484,6 +492,7 @@ int launch_kv8_rows(const Kv8Attn& a, int kind, int dh, int ctas, cudaStream_t s
   return dh == 64 ? launch_rows<KV8_E4M3, 64>(a, ctas, st) : launch_rows<KV8_E4M3, 128>(a, ctas, st);
 }
 int kv8_rows_tile() { return KB_ROWS; }
+int kv8_rows_places() { return KB_PLACES; }
 int kv8_rows_share() { return KB_SHARE; }
 int kv8_rows_extra() { return KB_EXTRA; }
 

@@ -403,6 +403,73 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
   }
 }
 
+// Tiles that lie in more than one CTA: the CTA behind the tile's first boundary has its block here.  The warps take the
+// parts in turn.
+constexpr int KM_WARPS = 16;
+template <int DH>
+__global__ void __launch_bounds__(32 * KM_WARPS) kv8_attn_merge_kernel(const __grid_constant__ Kv8Attn a) {
+  constexpr int QR = KA_ROWS, PER = DH / 32;
+  __shared__ float s_max[KM_WARPS], s_sum[KM_WARPS];
+  __shared__ float s_o[KM_WARPS][DH];
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // the parts are complete
+  const int b = blockIdx.x + 1;
+  const Kv8Desc d = a.desc[b];
+  const long long at = static_cast<long long>(d.share) * b;
+  // starts here, ends before, or has begun before the last boundary
+  if (at >= d.units || d.lo >= at || d.hi <= at || d.lo < at - d.share) return;
+  const int parts = static_cast<int>((d.hi - at + d.share - 1) / d.share) + 1;
+  const size_t s0 = static_cast<size_t>(b - 1) * 2 + (d.lo == at - d.share ? 0 : 1);
+  auto slot = [&](int i) { return i == 0 ? s0 : static_cast<size_t>(b - 1 + i) * 2; };
+  const Kv8Entry x = kv8_entry(a, d.entry);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int base = d.tile * QR, n_rows = min(QR, x.rows * a.group - base);
+  const int ctx = min(x.ctx, a.c.max_pages * KV8_PAGE);
+  // warp w has row w mod n_rows, and of its parts every subs-th from w / n_rows on
+  const int r = warp % n_rows, sub = warp / n_rows, subs = KM_WARPS / n_rows;
+  const int mine = sub < subs && sub < parts ? (parts - sub + subs - 1) / subs : 0;
+  auto ml = [&](int i) { return *reinterpret_cast<const float2*>(a.part_ml + (slot(sub + subs * i) * QR + r) * 2); };
+  float gm = -INFINITY, gl = 0.f, o[PER];
+  for (int i = lane; i < mine; i += 32) gm = fmaxf(gm, ml(i).x);
+  gm = warp_max(gm);
+  if (lane == 0) s_max[warp] = gm;
+#pragma unroll
+  for (int y = 0; y < PER; ++y) o[y] = 0.f;
+  __syncthreads();
+  for (int w = r; w < subs * n_rows; w += n_rows) gm = fmaxf(gm, s_max[w]);
+  for (int i0 = 0; i0 < mine; i0 += 32) {
+    float k = 0.f;
+    if (i0 + lane < mine) {
+      const float2 v = ml(i0 + lane);
+      k = part_weight(v.x, v.y, gm);
+      if (k != 0.f) gl += k * v.y;
+    }
+    const int n = min(32, mine - i0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float ki = __shfl_sync(0xffffffffu, k, i);
+      const float* src = a.part_o + (slot(sub + subs * (i0 + i)) * QR + r) * DH + lane * PER;
+#pragma unroll
+      for (int y = 0; y < PER; ++y) o[y] = fmaf(ki, src[y], o[y]);
+    }
+  }
+  gl = warp_sum(gl);
+  if (lane == 0) s_sum[warp] = gl;
+#pragma unroll
+  for (int y = 0; y < PER; ++y) s_o[warp][lane * PER + y] = o[y];
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_rows * DH; e += 32 * KM_WARPS) {
+    const int er = e / DH, ch = e % DH, rr = base + er;
+    float v = 0.f, sum = 0.f;
+    for (int w = er; w < subs * n_rows; w += n_rows) {
+      v += s_o[w][ch];
+      sum += s_sum[w];
+    }
+    const bool any = ctx - x.rows + rr / a.group + 1 > 0;
+    a.out[static_cast<size_t>(x.first + rr / a.group) * a.ldo + (d.head * a.group + rr % a.group) * DH + ch] =
+        __float2bfloat16(any ? v / sum : 0.f);
+  }
+}
+
 template <int KIND, int DH>
 static int launch_attn(const Kv8Attn& a, int ctas, cudaStream_t st) {
   using S = Kv8Smem<DH>;
@@ -415,7 +482,7 @@ static int launch_attn(const Kv8Attn& a, int ctas, cudaStream_t st) {
     if (dev < 64) set[dev] = true;
   }
   kv8_attn_kernel<KIND, DH><<<ctas, 32, S::BYTES, st>>>(a);
-  const int rc = launch_kv8_merge<DH, KA_ROWS>(a, ctas, st);
+  const int rc = launch_kv8_merge(kv8_attn_merge_kernel<DH>, dim3(ctas - 1), 32 * KM_WARPS, a, ctas, st);
   if (rc != 0) return rc;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

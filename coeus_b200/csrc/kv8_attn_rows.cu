@@ -252,60 +252,71 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
       }
     }
   } else if (warp == 8) {
-    // ---- scores, issued by one thread
-    if (elect_one()) {
-      constexpr uint32_t id_s = idesc_f16(KB_ROWS, KV8_PAGE);
-      const uint64_t dq = umma_desc_sw128(smem_u32(sq), 16, 1024), dk = umma_desc_sw128(smem_u32(stage), 16, 1024);
-      int gi = 0, tiles = 0;
-      for (int u = u0; u < u1 && !dead;) {
-        const Piece t = piece_at(u);
-        u = next_tile(t);
-        if (!t.any || t.p0 >= t.p1) continue;
-        wait(q_full, tiles++);
-        for (int n = t.p1 - t.p0; n > 0; --n, ++gi) {
-          const int st = gi % KB_STAGES;
-          wait(full + st, gi / KB_STAGES);
-          if (gi >= 2) wait(o_done + (gi & 1), (gi >> 1) - 1);   // the weights that were here have been used
-          if (dead) break;
-          tc_fence_after();
-          const uint64_t dks = dk + st * (S::STAGE >> 4);
-          const uint32_t d = tmem + KB_S + (gi & 1) * KV8_PAGE;
+    // ---- scores: the warp goes through the loop together (its addresses then are uniform registers, which the
+    // instruction wants) and one thread of it issues
+    constexpr uint32_t id_s = idesc_f16(KB_ROWS, KV8_PAGE);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t dq = umma_desc_sw128(smem_u32(sq), 16, 1024), dk = umma_desc_sw128(smem_u32(stage), 16, 1024);
+    int gi = 0, tiles = 0;
+    for (int u = u0; u < u1 && !dead;) {
+      const Piece t = piece_at(u);
+      u = next_tile(t);
+      if (!t.any || t.p0 >= t.p1) continue;
+      wait(q_full, tiles++);
+      for (int n = t.p1 - t.p0; n > 0; --n, ++gi) {
+        const int st = gi % KB_STAGES;
+        wait(full + st, gi / KB_STAGES);
+        if (gi >= 2) wait(o_done + (gi & 1), (gi >> 1) - 1);     // the weights that were here have been used
+        if (__any_sync(0xffffffffu, dead)) {
+          dead = true;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t dks = dk + static_cast<uint64_t>(st * (S::STAGE >> 4));
+        const uint32_t d = tm + KB_S + (gi & 1) * KV8_PAGE;
+        if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < HALVES; ++h)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_bf16_ss(d, dq + ((h * KB_ROWS * 128 + k * 32) >> 4), dks + ((h * S::PANEL_K + k * 32) >> 4), id_s, h + k > 0 ? 1u : 0u);
+              umma_bf16_ss(d, dq + static_cast<uint64_t>((h * KB_ROWS * 128 + k * 32) >> 4),
+                           dks + static_cast<uint64_t>((h * S::PANEL_K + k * 32) >> 4), id_s, h + k > 0 ? 1u : 0u);
           umma_commit(smem_u32(s_full + (gi & 1)));
+          if (n == 1) umma_commit(smem_u32(q_free));
         }
-        umma_commit(smem_u32(q_free));
+        __syncwarp();
       }
     }
-    __syncwarp();
   } else if (warp == 9) {
     // ---- weighted values
-    if (elect_one()) {
-      constexpr uint32_t id_o = idesc_f16(KB_ROWS, DH);
-      const uint64_t dv = umma_desc_sw128(smem_u32(stage + S::V), 16, 1024);
-      int gi = 0;
-      for (int u = u0; u < u1 && !dead;) {
-        const Piece t = piece_at(u);
-        u = next_tile(t);
-        if (!t.any) continue;
-        for (int p = t.p0; p < t.p1; ++p, ++gi) {
-          wait(p_full + (gi & 1), gi >> 1);
-          if (dead) break;
-          tc_fence_after();
-          const int st = gi % KB_STAGES;
-          const uint64_t dvs = dv + st * (S::STAGE >> 4);
-          const uint32_t pa = tmem + KB_S + (gi & 1) * KV8_PAGE;
+    constexpr uint32_t id_o = idesc_f16(KB_ROWS, DH);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t dv = umma_desc_sw128(smem_u32(stage + S::V), 16, 1024);
+    int gi = 0;
+    for (int u = u0; u < u1 && !dead;) {
+      const Piece t = piece_at(u);
+      u = next_tile(t);
+      if (!t.any) continue;
+      for (int p = t.p0; p < t.p1; ++p, ++gi) {
+        wait(p_full + (gi & 1), gi >> 1);
+        if (__any_sync(0xffffffffu, dead)) {
+          dead = true;
+          break;
+        }
+        tc_fence_after();
+        const int st = gi % KB_STAGES;
+        const uint64_t dvs = dv + static_cast<uint64_t>(st * (S::STAGE >> 4));
+        const uint32_t pa = tm + KB_S + (gi & 1) * KV8_PAGE;
+        const uint32_t more = p > t.p0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ts(tmem + KB_O, pa + k * 8, dvs + ((k * 32) >> 4), id_o, k > 0 || p > t.p0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) umma_bf16_ts(tm + KB_O, pa + k * 8, dvs + static_cast<uint64_t>((k * 32) >> 4), id_o, k > 0 ? 1u : more);
           umma_commit(smem_u32(o_done + (gi & 1)));
           umma_commit(smem_u32(empty + st));
         }
+        __syncwarp();
       }
     }
-    __syncwarp();
   } else {
     // ---- weights: a row per thread
     const uint32_t mine = tmem + (static_cast<uint32_t>(warp * 32) << 16);
@@ -467,6 +478,43 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
   }
 }
 
+// Tiles that lie in more than one CTA, as in kv8_attn.cuh, for tiles of many rows and few parts: a warp a row.
+template <int DH>
+__global__ void __launch_bounds__(256) kv8_rows_merge_kernel(const __grid_constant__ Kv8Attn a) {
+  constexpr int PER = DH / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // the parts are complete
+  const int b = blockIdx.x + 1;
+  const Kv8Desc d = a.desc[b];
+  const long long at = static_cast<long long>(d.share) * b;
+  if (at >= d.units || d.lo >= at || d.hi <= at || d.lo < at - d.share) return;
+  const int parts = static_cast<int>((d.hi - at + d.share - 1) / d.share) + 1;
+  const Kv8Entry x = kv8_entry(a, d.entry);
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, rr = d.tile * KB_ROWS + r;
+  if (rr >= x.rows * a.group) return;
+  const size_t s0 = static_cast<size_t>(b - 1) * 2 + (d.lo == at - d.share ? 0 : 1);
+  auto slot = [&](int i) { return (i == 0 ? s0 : static_cast<size_t>(b - 1 + i) * 2) * KB_ROWS + r; };
+  float gm = -INFINITY, gl = 0.f, o[PER];
+  for (int i = lane; i < parts; i += 32) gm = fmaxf(gm, a.part_ml[slot(i) * 2]);
+  gm = warp_max(gm);
+#pragma unroll
+  for (int y = 0; y < PER; ++y) o[y] = 0.f;
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    const float2 v = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
+    const float k = part_weight(v.x, v.y, gm);
+    const float* src = a.part_o + slot(i) * DH + lane * PER;
+    if (k != 0.f) gl += k * v.y;
+#pragma unroll
+    for (int y = 0; y < PER; ++y) o[y] = fmaf(k, src[y], o[y]);
+  }
+  const int ctx = min(x.ctx, a.c.max_pages * KV8_PAGE);
+  const float inv = ctx - x.rows + rr / a.group + 1 > 0 ? 1.f / gl : 0.f;
+  __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(
+      a.out + static_cast<size_t>(x.first + rr / a.group) * a.ldo + (d.head * a.group + rr % a.group) * DH + lane * PER);
+#pragma unroll
+  for (int y = 0; y < PER; y += 2) dst[y / 2] = __floats2bfloat162_rn(o[y] * inv, o[y + 1] * inv);
+}
+
 static_assert(RowsSmem<128>::BYTES <= 113 * 1024 && KB_PLACES * KB_COLS <= 512, "two CTAs per SM");
 
 template <int KIND, int DH>
@@ -483,7 +531,7 @@ static int launch_rows(const Kv8Attn& a, int ctas, cudaStream_t st) {
     if (dev < 64) set[dev] = true;
   }
   kv8_rows_kernel<KIND, DH><<<ctas, KB_THREADS, bytes, st>>>(a);
-  const int rc = launch_kv8_merge<DH, KB_ROWS>(a, ctas, st);
+  const int rc = launch_kv8_merge(kv8_rows_merge_kernel<DH>, dim3(ctas - 1, KB_ROWS / 8), 256, a, ctas, st);
   if (rc != 0) return rc;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

@@ -21,8 +21,8 @@ namespace cb {
 constexpr int BEAM_MAX = 32;           // beams of a request
 constexpr int BLK = 512;               // logits of a block (ops/beam.py sizes the scratch by it)
 constexpr int PICK_THREADS = 512;
-constexpr int PICK_PER = 6;            // blocks that a thread keeps the values of
-constexpr int PICK_CAP = 1024;         // continuations compared at once
+constexpr int PICK_PER = 4;            // blocks that a thread keeps the values of
+constexpr int PICK_CAP = 1024;         // continuations compared at once; at least BEAM_MAX for every warp
 
 // Blocks begin at multiples of 16 bytes, so that a row that does not is read in vectors all the same: block k of a row
 // whose first logit is `skew` logits behind such a place has logits k BLK - skew .. (k + 1) BLK - skew - 1, as far as
@@ -81,15 +81,22 @@ __global__ void __launch_bounds__(32 * PASS_WARPS) beam_pass_kernel(const T* __r
 }
 
 struct Best {              // a continuation or a block: larger value first, then the lower place
-  double v;
-  int64_t at;
+  int64_t v;               // key of the value
+  uint32_t at;             // at most 32 beams of 2^26 logits
 };
-__device__ __forceinline__ bool better(double v, int64_t at, const Best& b) { return v > b.v || (v == b.v && at < b.at); }
+// Values as whole numbers in the same order (-0 below +0, which the sums here never give): comparing these takes a
+// tenth of what fp64 comparisons do, and the selection is little else.
+__device__ __forceinline__ int64_t value_key(double v) {
+  const int64_t b = __double_as_longlong(v + 0.0);
+  return b ^ ((b >> 63) & 0x7fffffffffffffffll);
+}
+__device__ __forceinline__ double key_value(int64_t k) { return __longlong_as_double(k ^ ((k >> 63) & 0x7fffffffffffffffll)); }
+__device__ __forceinline__ bool better(int64_t v, uint32_t at, const Best& b) { return v > b.v || (v == b.v && at < b.at); }
 __device__ __forceinline__ Best block_best(Best b, Best* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const double v = __shfl_xor_sync(0xffffffffu, b.v, o);
-    const int64_t at = __shfl_xor_sync(0xffffffffu, b.at, o);
+    const int64_t v = __shfl_xor_sync(0xffffffffu, b.v, o);
+    const uint32_t at = __shfl_xor_sync(0xffffffffu, b.at, o);
     if (better(v, at, b)) b = Best{v, at};
   }
   __syncthreads();
@@ -108,24 +115,33 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
                  float* __restrict__ out_score, int64_t* __restrict__ out_parent, int64_t* __restrict__ out_token,
                  uint8_t* __restrict__ out_done) {
   __shared__ Best red[PICK_THREADS / 32];
-  __shared__ double s_lse[BEAM_MAX];
-  __shared__ int64_t s_blk[BEAM_MAX];
-  __shared__ double c_v[PICK_CAP];
-  __shared__ int64_t c_at[PICK_CAP];
+  enum : int { DEAD, LIVE, ENDED };
+  __shared__ double s_lse[BEAM_MAX], s_score[BEAM_MAX];
+  __shared__ int s_state[BEAM_MAX];
+  __shared__ int s_blk[BEAM_MAX];
+  __shared__ int64_t c_v[PICK_CAP];
+  __shared__ uint32_t c_at[PICK_CAP];
+  __shared__ int64_t s_least;
   __shared__ int s_n;
   const int item = blockIdx.x, row0 = item * K;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const double NEG = -INFINITY;
+  const int64_t NEG = value_key(-INFINITY), TOP = 0x7fffffffffffffffll;
+  constexpr uint32_t NONE = 0xffffffffu;
   for (int j = warp; j < K; j += PICK_THREADS / 32) {
     const float2* p = part + static_cast<size_t>(row0 + j) * nblk;
-    double lse = NEG;
-    if (!done[row0 + j] && scores[row0 + j] != -INFINITY) {
+    // scores and states once, in shared memory: what follows asks for them all the time
+    const float score = scores[row0 + j];
+    const int state = done[row0 + j] ? ENDED : score != -INFINITY ? LIVE : DEAD;
+    double lse = -INFINITY;
+    if (state == LIVE) {
       // in fp64 but for the factors of the blocks: their errors (2 units of fp32 each) average out like those of the
       // logits' own exponentials
       float m = -INFINITY;
+#pragma unroll 4
       for (int i = lane; i < nblk; i += 32) m = fmaxf(m, p[i].x);
       m = warp_max(m);
       double s = 0.0;
+#pragma unroll 1
       for (int i = lane; i < nblk; i += 32) {
         const float2 q = p[i];
         s += q.x == -INFINITY && q.y == 0.f ? 0.0 : static_cast<double>(q.y) * static_cast<double>(expf(q.x - m));
@@ -134,64 +150,110 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       lse = static_cast<double>(m) + log(s);
     }
-    if (lane == 0) s_lse[j] = lse;
+    if (lane == 0) {
+      s_lse[j] = lse;
+      s_score[j] = static_cast<double>(score);
+      s_state[j] = state;
+    }
   }
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
   // the value of a logit of beam j; what is not a number is no continuation
   auto value = [&](int j, float x) {
-    const double v = static_cast<double>(scores[row0 + j]) + (static_cast<double>(x) - s_lse[j]);
-    return v == v ? v : NEG;
+    const double v = s_score[j] + (static_cast<double>(x) - s_lse[j]);
+    return v == v ? value_key(v) : NEG;
   };
-  // the K best blocks, one after the other; an ended beam is one block
-  auto block_value = [&](int i) {
-    const int j = i / nblk, k = i % nblk;
-    double v = NEG;
-    if (done[row0 + j]) {
-      if (k == 0 && eos >= 0) v = scores[row0 + j];
-      if (v != v) v = NEG;
-    } else if (scores[row0 + j] != -INFINITY) {
-      v = value(j, part[static_cast<size_t>(row0 + j) * nblk + k].x);
+  // the K best blocks (an ended beam is one block): each warp the K best of its share, one after the other without the
+  // other warps, then every one of these counts those before it
+  auto block_value = [&](int i, float x) {                       // x: the block's maximum
+    const int j = i / nblk;
+    if (s_state[j] == LIVE) return value(j, x);
+    return s_state[j] == ENDED && i == j * nblk && eos >= 0 && s_score[j] == s_score[j] ? value_key(s_score[j]) : NEG;
+  };
+  const float2* row_part = part + static_cast<size_t>(row0) * nblk;
+  {
+    int64_t mine[PICK_PER];                                      // a thread keeps its first ones
+    float top[PICK_PER];
+#pragma unroll
+    for (int u = 0; u < PICK_PER; ++u) {
+      const int i = threadIdx.x + u * PICK_THREADS;
+      top[u] = i < K * nblk && s_state[i / nblk] == LIVE ? row_part[i].x : 0.f;
     }
-    return v;
-  };
-  int found = 0;
-  Best last{INFINITY, -1};
-  double mine[PICK_PER];                                         // a thread keeps its first ones
 #pragma unroll
-  for (int u = 0; u < PICK_PER; ++u) {
-    const int i = threadIdx.x + u * PICK_THREADS;
-    mine[u] = i < K * nblk ? block_value(i) : NEG;
+    for (int u = 0; u < PICK_PER; ++u) {
+      const int i = threadIdx.x + u * PICK_THREADS;
+      mine[u] = i < K * nblk ? block_value(i, top[u]) : NEG;
+    }
+    Best last{TOP, NONE};
+    for (int n = 0; n < K; ++n) {
+      Best b{NEG, NONE};
+      auto look = [&](int64_t v, uint32_t i) {
+        if (v > NEG && better(v, i, b) && !better(v, i, last) && i != last.at) b = Best{v, i};
+      };
+#pragma unroll
+      for (int u = 0; u < PICK_PER; ++u) look(mine[u], threadIdx.x + u * PICK_THREADS);
+      for (int i = threadIdx.x + PICK_PER * PICK_THREADS; i < K * nblk; i += PICK_THREADS)
+        look(block_value(i, s_state[i / nblk] == LIVE ? row_part[i].x : 0.f), i);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const int64_t v = __shfl_xor_sync(0xffffffffu, b.v, o);
+        const uint32_t at = __shfl_xor_sync(0xffffffffu, b.at, o);
+        if (better(v, at, b)) b = Best{v, at};
+      }
+      if (lane == 0) {
+        c_v[warp * K + n] = b.v;
+        c_at[warp * K + n] = b.at;
+      }
+      last = b;
+      if (!(b.v > NEG)) last.v = NEG;                            // no more: so will be the others
+    }
   }
-  for (; found < K; ++found) {
-    Best b{NEG, 0x7fffffffffffffffll};
-    auto look = [&](double v, int i) {
-      if (v > NEG && better(v, i, b) && !better(v, i, last) && i != last.at) b = Best{v, i};
-    };
-#pragma unroll
-    for (int u = 0; u < PICK_PER; ++u) look(mine[u], threadIdx.x + u * PICK_THREADS);
-    for (int i = threadIdx.x + PICK_PER * PICK_THREADS; i < K * nblk; i += PICK_THREADS) look(block_value(i), i);
-    b = block_best(b, red);
-    if (!(b.v > NEG)) break;
-    if (threadIdx.x == 0) s_blk[found] = b.at;
-    last = b;
+  if (threadIdx.x < K) s_blk[threadIdx.x] = -1;
+  __syncthreads();
+  const int warp_best = PICK_THREADS / 32 * K;
+  for (int i = threadIdx.x; i < warp_best; i += PICK_THREADS) {
+    const Best me{c_v[i], c_at[i]};
+    if (!(me.v > NEG)) continue;
+    int rank = 0;
+#pragma unroll 8
+    for (int o = 0; o < warp_best; ++o) rank += better(c_v[o], c_at[o], me);
+    if (rank < K) {
+      s_blk[rank] = static_cast<int>(me.at);
+      if (rank == K - 1) s_least = me.v;
+    }
   }
   __syncthreads();
-  const double least = found == K ? last.v : NEG;
-  // every continuation of those blocks that is not below the last block's best
-  auto each = [&](auto&& f) {
-    for (int n = 0; n < found; ++n) {
-      const int j = static_cast<int>(s_blk[n] / nblk), k = static_cast<int>(s_blk[n] % nblk);
-      if (done[row0 + j]) {
-        if (threadIdx.x == 0) f(static_cast<double>(scores[row0 + j]), static_cast<int64_t>(j) * V + eos);
+  int found = 0;
+  while (found < K && s_blk[found] >= 0) ++found;
+  const int64_t least = found == K ? s_least : NEG;
+  // every continuation of those blocks that is not below the last block's best: a warp a block
+  auto each = [&](int64_t floor, auto&& f) {
+    for (int n = warp; n < found; n += PICK_THREADS / 32) {
+      const int j = s_blk[n] / nblk, k = s_blk[n] % nblk;
+      if (s_state[j] == ENDED) {
+        if (lane == 0) f(value_key(s_score[j]), static_cast<uint32_t>(j) * V + eos);
         continue;
       }
       const T* x = logits + (row0 + j) * ld;
-      const int t0 = k * BLK - beam_skew(x);
-      for (int t = max(0, t0) + threadIdx.x; t < min(V, t0 + BLK); t += PICK_THREADS) f(value(j, beam_logit(x + t)), static_cast<int64_t>(j) * V + t);
+      const int t0 = k * BLK - beam_skew(x) + lane;
+      x += t0;
+      float v[BLK / 32];
+#pragma unroll
+      for (int i = 0; i < BLK / 32; ++i) v[i] = t0 + 32 * i >= 0 && t0 + 32 * i < V ? beam_logit(x + 32 * i) : -INFINITY;
+      // few of them count: the others are told by their logit alone
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < BLK / 32; ++i) top = fmaxf(top, v[i]);
+      if (value(j, top) < floor) continue;
+#pragma unroll 1
+      for (int i = 0; i < BLK / 32; ++i) {
+        const int t = t0 + 32 * i;
+        if (t >= 0 && t < V) f(value(j, beam_logit(x + 32 * i)), static_cast<uint32_t>(j) * V + t);
+      }
     }
   };
-  each([&](double v, int64_t at) {
+  __syncthreads();                       // the list is used again
+  each(least, [&](int64_t v, uint32_t at) {
     if (v >= least && v > NEG) {
       const int n = atomicAdd(&s_n, 1);
       if (n < PICK_CAP) {
@@ -202,12 +264,12 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
   });
   __syncthreads();
   const int n = s_n;
-  auto put = [&](int place, double v, int64_t at) {
-    const int j = static_cast<int>(at / V), t = static_cast<int>(at % V);
-    out_score[row0 + place] = static_cast<float>(v);
+  auto put = [&](int place, int64_t v, uint32_t at) {
+    const int j = static_cast<int>(at / static_cast<uint32_t>(V)), t = static_cast<int>(at - static_cast<uint32_t>(j) * V);
+    out_score[row0 + place] = static_cast<float>(key_value(v));
     out_parent[row0 + place] = j;
     out_token[row0 + place] = t;
-    out_done[row0 + place] = done[row0 + j] || t == eos;
+    out_done[row0 + place] = s_state[j] == ENDED || t == eos;
   };
   int filled;
   if (n <= PICK_CAP) {
@@ -221,10 +283,10 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
     filled = min(n, K);
   } else {
     // more equal ones than that: one after the other
-    Best prev{INFINITY, -1};
+    Best prev{TOP, NONE};
     for (filled = 0; filled < K; ++filled) {
-      Best b{NEG, 0x7fffffffffffffffll};
-      each([&](double v, int64_t at) {
+      Best b{NEG, NONE};
+      each(NEG, [&](int64_t v, uint32_t at) {
         if (v > NEG && better(v, at, b) && !better(v, at, prev) && at != prev.at) b = Best{v, at};
       });
       b = block_best(b, red);

@@ -28,7 +28,7 @@ __device__ __forceinline__ bool kv8_piece(const Kv8Cache& c, const Kv8Rows& r, i
   int n = r.row0 != nullptr ? r.row0[e + 1] - first : 1;
   const int pos0 = r.pos0[e];
   if (n <= 0) return false;
-  if (n > r.most || first < 0 || first + n > r.rows || pos0 < 0) {
+  if (n > r.most || first < 0 || n > r.rows - first || pos0 < 0 || pos0 > 0x7fffffff - n - KV8_PAGE) {
     record_status(status, ST_BOUNDS, e);
     return false;
   }

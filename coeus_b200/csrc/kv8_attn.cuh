@@ -83,7 +83,7 @@ __device__ __forceinline__ Kv8Entry kv8_entry(const Kv8Attn& a, int e) {
   x.rows = a.row0 != nullptr ? a.row0[e + 1] - x.first : 1;
   x.ctx = max(0, a.ctx[e]);
   if (x.rows <= 0) x.rows = 0;
-  else if (x.rows > a.most || x.first < 0 || x.first + x.rows > a.rows) x.rows = -1;
+  else if (x.rows > a.most || x.first < 0 || x.rows > a.rows - x.first) x.rows = -1;
   return x;
 }
 

@@ -55,8 +55,8 @@ def _check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, ints, row0
         raise ValueError(f"{what}: keys are [pages, heads, dh / 64, {PAGE}, 64] codes, got "
                          f"{tuple(shape)} {dtype}")
     pages, heads, dh = shape[0], shape[1], shape[2] * 64
-    if dh != 64 and dh != 128:
-        raise ValueError(f"{what}: heads of 64 or 128, not {dh}")
+    if (dh != 64 and dh != 128) or heads < 1 or pages < 1:
+        raise ValueError(f"{what}: pages and heads of 64 or 128, not {tuple(shape)}")
     if v_cache.shape != (pages, heads, dh, PAGE) or v_cache.dtype != dtype:
         raise ValueError(f"{what}: values {tuple(v_cache.shape)} {v_cache.dtype} do not go with "
                          f"keys {tuple(shape)} {dtype}")
@@ -182,8 +182,8 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                 k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k_cache.data_ptr(),
                 v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
                 page_table.shape[1], pages, heads, dh, int(k_cache.dtype != torch.int8),
-                None if row0 is None else row0.data_ptr(), pos0.data_ptr(), n, rows, max_rows,
-                _status(device), _lib.stream_int())
+                None if row0 is None else row0.data_ptr(), pos0.data_ptr(), n, rows,
+                min(max_rows, rows), _status(device), _lib.stream_int())
         _lib.check_rc(rc, "cb_kv8_write")
         return
     dtype = k_cache.dtype
@@ -239,7 +239,7 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
                     k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
                     v_scale.data_ptr(), page_table.data_ptr(), page_table.shape[1], pages, heads,
                     dh, int(k_cache.dtype != torch.int8), row0.data_ptr(), pos0.data_ptr(), n,
-                    rows, max_rows, k.data_ptr(), v.data_ptr(), heads * dh, _status(device),
+                    rows, min(max_rows, rows), k.data_ptr(), v.data_ptr(), heads * dh, _status(device),
                     _lib.stream_int())
             _lib.check_rc(rc, "cb_kv8_read")
         return k, v
@@ -290,7 +290,9 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                                       device=q.device)
         if n == 0 or rows == 0:
             return out
-        width = page_table.shape[1]
+        width, max_rows = page_table.shape[1], min(max_rows, rows)
+        if width * PAGE >= 1 << 31:
+            raise ValueError(f"kv8_attention: page tables of {width} pages")
         with _lib.on_device(device):
             scratch = torch.empty(_scratch(n, rows, max_rows, nh // heads, width, heads, dh),
                                   dtype=torch.uint8, device=q.device)

@@ -79,6 +79,8 @@ def test_refusals():
     refused(v_cache=v[:, :1])
     refused(v_cache=v.view(torch.float8_e4m3fn))
     refused(k_cache=k.float())
+    refused(k_cache=k[:0], v_cache=v[:0], k_scale=ks[:0], v_scale=vs[:0])
+    refused(k_cache=k[:, :0], v_cache=v[:, :0], k_scale=ks[:, :0], v_scale=vs[:, :0], k=x[:, :0], v=x[:, :0])
     refused(k_scale=ks.double())
     refused(page_table=c.table.long())
     refused(page_table=c.table.t().contiguous().t())

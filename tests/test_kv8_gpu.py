@@ -265,6 +265,71 @@ def test_rows_without_entry_and_bad_entries():
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+def test_numbers_at_the_edge():
+    """Positions next to 2^31, an unbounded max_rows, more entries than one launch takes, an entry
+    whose row numbers wrap around."""
+    c = Case("int8", 1, 64, [3, 3], DEV)
+    k = torch.randn(2, 64, device=DEV).bfloat16()
+    table = c.table.to(DEV)
+    kv8.kv8_write(k, k, *c.c, table, i32([2 ** 31 - 1, 2 ** 31 - 40], DEV))
+    assert status() == 2
+    kv8.kv8_write(k, k, *c.c, table, i32([0, 0], DEV), row0=i32([0, 1, 2], DEV), max_rows=2 ** 40)
+    out = kv8.kv8_attention(k, *c.c, table, i32([1, 1], DEV), 1, row0=i32([0, 1, 2], DEV), max_rows=2 ** 40)
+    assert status() == 0
+    got, _ = kv8.kv8_read(*c.c, table, i32([0, 0], DEV), i32([0, 1, 2], DEV), 2, 2 ** 40)
+    assert (got.float() - k.float()).abs().max() < 0.1 and (out.float() - k.float()).abs().max() < 0.1
+    kv8.kv8_attention(k, *c.c, table, i32([1, 1], DEV), 1, row0=i32([-2 ** 31, 2 ** 31 - 1, 2], DEV), max_rows=2)
+    assert status() in (0, 2)
+    kv8.kv8_write(k, k, *c.c, table, i32([0, 0], DEV), row0=i32([2, 2 ** 31 - 1, 0], DEV), max_rows=2 ** 31)
+    assert status() == 2
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_more_entries_than_a_launch_takes(rows):
+    n = 600
+    lens = [60 + (i * 37) % 70 for i in range(n)]
+    c = Case("e4m3", 1, 64, lens, DEV)
+    c.write([0] * n, lens)
+    c.check_attend(lens, [rows] * n if rows == 1 else [rows if i % 100 == 3 else i % 3 for i in range(n)], 2)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_wide_tiles(kind):
+    """Many rows: tiles that end inside a page, heads that do not divide them, several tiles of several
+    entries in every block, contexts split over blocks, pages without values, and scales apart."""
+    c = Case(kind, 3, 128, [700, 2500, 65, 0, 1500], DEV)
+
+    def edit(k, v):
+        v[64:128] = 0.0                                    # entry 0, page 1: no values
+        k[128:192] = 0.0
+        v[700 + 64:700 + 128] *= 2.0 ** 20                 # entry 1, page 1
+        v[700 + 640:700 + 704] *= 2.0 ** -25
+    c.write([0] * 5, [700, 2500, 65, 0, 1500], edit=edit)
+    c.check_attend([700, 2500, 65, 0, 1500], [333, 57, 65, 0, 129], 15)
+    c.check_attend([699, 2500, 3, 0, 64], [50, 1, 65, 0, 64], 3)
+    got = [c.attend(torch.ones(130, 3 * 128).bfloat16(), [700, 2500, 65, 0, 1500], [60, 1, 2, 0, 67], 3) for _ in range(3)]
+    assert all(torch.equal(x, got[0]) for x in got)
+    assert status() == 0
+
+
+def test_wide_tiles_not_a_number():
+    c = Case("e4m3", 2, 64, [300], DEV)
+
+    def edit(k, v):
+        k[70, 3] = math.nan                                # page 1, head 0: keys
+        v[140, 64 + 9] = math.inf                          # page 2, head 1: values
+    c.write([0], [300], edit=edit)
+    o = c.check_attend([300], [280], 2)                    # rows 0 .. 43 do not see page 1
+    assert not torch.isnan(o[:44, :64]).any() and torch.isnan(o[44:, :64]).all()
+    assert not torch.isnan(o[:108, 64:]).any() and torch.isnan(o[108:, 64:]).all()
+    page = int(c.table[0, 4])
+    c.c[1].view(torch.int8)[page, :, :, 44:] = 127         # behind the context: NaN codes
+    c.c[0].view(torch.int8)[page, :, :, 44:] = 127
+    c.check_attend([300], [100], 2)
+    assert status() == 0
+
+
 def test_gpu_refusals():
     c = Case("int8", 1, 64, [3], DEV)
     x = torch.zeros(1, 64, device=DEV)

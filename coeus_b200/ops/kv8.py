@@ -316,10 +316,14 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         x = q[r0:r0 + cnt].float().view(cnt, heads, g, dh)
         s = torch.einsum("rhgd,hcd->hgrc", x, K) * scale
         seen = torch.arange(c)[None] <= (c - cnt + torch.arange(cnt))[:, None]       # [rows, c]
-        # values a row does not see stay out of its sum, whatever they are
         w = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
         w = torch.where(seen, w, torch.zeros_like(w))
-        o = torch.einsum("hgrc,hcd->rhgd", w, V)
+        # a value that is NaN counts for the rows that see it and no others
+        none = torch.isnan(V)
+        o = torch.einsum("hgrc,hcd->rhgd", w, V.masked_fill(none, 0.0))
+        if none.any():
+            hit = torch.einsum("rc,hcd->rhd", seen.float(), none.float()) > 0
+            o = o.masked_fill(hit[:, :, None], math.nan)
         o = torch.where(seen.any(-1)[:, None, None, None], o, torch.zeros_like(o))
         out[r0:r0 + cnt] = o.reshape(cnt, -1).to(q.dtype)
     return out

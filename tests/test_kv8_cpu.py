@@ -47,6 +47,9 @@ def test_not_a_number_makes_its_block_one(kind):
     k, v = c.read([0], [130])
     assert torch.isnan(k[:64, :64]).all() and not torch.isnan(k[64:]).any()
     assert torch.isnan(v[64:128, 64:]).all() and not torch.isnan(v[:64]).any()
+    # rows count what they see: the first two of four rows end in front of page 1
+    o = c.check_attend([66], [4], 2)
+    assert not torch.isnan(o[:2, 64:]).any() and torch.isnan(o[2:, 64:]).all()
     c.write([0], [130])                                    # from its first token on a page is new
     c.check_read([0], [130])
 

@@ -30,9 +30,13 @@ namespace cb {
 constexpr int KA_ROWS = 8;                        // query rows of a tile
 constexpr int KA_SHARE = 2;                       // units a CTA takes at least
 constexpr int KA_EXTRA = 1;                       // what a tile costs beside its pages, in units
-// Rows and heads of an entry that share a key/value head: more take the wide tiles.  36 of them (24 sequences, 500 to
-// 4100 tokens): 86 us here, 98 us there; 2800: 1909 and 469.
-constexpr int KA_WIDE = 48;
+// Rows and heads of an entry that share a key/value head: up to KA_NARROW this kernel's tiles are the faster ones, above
+// KA_WIDE the wide ones.  In between a tile of eight more costs 2.6 ns a page here (dh 128, the device full) and nothing
+// there, where a page costs 5.7 ns and the call some 18 us more: wide when the tiles over two, times the pages, are more
+// than KA_WORK.  24 sequences of 500 to 4100 tokens, 8 heads, 24 / 32 / 48 / 64 rows: 82 / 100 / 137 / 172 us here, 80 / 82 /
+// 84 / 88 there; one sequence of 8000: 35 / 37 / 37 / 47 and 45 / 45 / 47 / 47, and
+// with 96 and 192 rows 51 / 84 and 51 / 53.
+constexpr int KA_NARROW = 24, KA_WIDE = 64, KA_WORK = 7000;
 constexpr int KA_BLOCK = 16;                      // units that are planned at a time
 constexpr int KA_RING = 4;                        // copies in a warp's ring: the keys and values of two pages
 constexpr int KA_PLACES = 6, KA_PLACES64 = 11;    // CTAs that share an SM, by its shared memory: dh 128, 64
@@ -495,7 +499,8 @@ struct AttnShape {
   long long units;
   AttnShape(int n, int rows, int most, int group, int max_pages, int kv_heads, int dh) {
     if (most > rows) most = rows;                              // a row counts at most once
-    wide = 1ll * most * group > KA_WIDE;
+    const long long shared = 1ll * most * group, pages = 1ll * n * kv_heads * max_pages;
+    wide = shared > KA_WIDE || (shared > KA_NARROW && ((shared + 7) / 8 - 2) * pages > KA_WORK);
     tile = wide ? kv8_rows_tile() : KA_ROWS;
     units = (1ll * most * group + tile - 1) / tile * (max_pages + (wide ? kv8_rows_extra() : KA_EXTRA)) * kv_heads;
     const long long fit = units > 0 ? 0x7fffffffll / units : 0;

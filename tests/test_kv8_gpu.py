@@ -313,6 +313,18 @@ def test_wide_tiles(kind):
     assert status() == 0
 
 
+@pytest.mark.parametrize("rows", [24, 25, 32, 33, 64])
+@pytest.mark.parametrize("width", [6, 5000])
+def test_tiles_by_rows_and_work(rows, width):
+    """On both sides of the bounds between the two tiles: of the rows, and of the pages that a table can name."""
+    lens = [300, 64, 129]
+    c = Case("int8", 2, 64, lens, DEV)
+    c.write([0] * 3, lens)
+    c.table = torch.cat([c.table, torch.full((3, width - c.table.shape[1]), -1, dtype=torch.int32)], 1)
+    c.check_attend(lens, [rows, 1, 7], 2)
+    assert status() == 0
+
+
 def test_wide_tiles_not_a_number():
     c = Case("e4m3", 2, 64, [300], DEV)
 

@@ -12,8 +12,11 @@
 // The scale 2^ev of a page's values goes into the weights: with z = s + ev (s the score in units of log2) and m a
 // running maximum of z, the weights are P = 2^(z - m), and the denominator sums 2^(e0 - ev) P, e0 the first page's ev:
 // o = 2^e0 sum P code / sum 2^(e0 - ev) P.  So pages of any scales add up in one accumulator.  The maximum is only
-// raised when z exceeds it by more than KB_LAG, and the sums so far are multiplied then.  Bound by the matrix products and the softmax between them: a page of a tile is 2 x 64 x 128 dh
-// multiply-adds and 8192 exponentials.
+// raised when z exceeds it by more than KB_LAG, and the sums so far are multiplied then.  A page of a tile is 2 x 64 x 128 dh
+// multiply-adds and 8192 exponentials; what bounds it is the chain of score product, softmax and value product, two tiles
+// an SM in turn.  Four sequences of 8192 with 512 rows each, 32 heads over 8 of 128: 448 us and 18 for the merge, 0.35 of
+// the bf16 rate.  Four of 2000 to 8200 with 301 to 700 rows: 351 us in all, 469 with one CTA an SM and one issuing thread;
+// 200 with nothing but the products and the barriers.  Keys and values handed over separately: 360.
 #include "kv8_attn.cuh"
 
 namespace cb {

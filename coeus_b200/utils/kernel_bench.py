@@ -53,7 +53,8 @@ def main(argv=None) -> int:
                                        "cross_entropy", "adamw", "decode_attn", "rope", "softmax",
                                        "swiglu", "gelu", "embed", "rmsnorm_fwd", "rmsnorm_bwd",
                                        "moe_route", "allreduce_local", "kv_write", "argmax",
-                                       "normal_init", "colsum", "moe_gather", "moe_combine"])
+                                       "normal_init", "colsum", "moe_gather", "moe_combine",
+                                       "kv8_write", "kv8_read", "kv8_attn", "beam_select"])
     ap.add_argument("--m", type=int, default=16384)
     ap.add_argument("--n", type=int, default=4096)
     ap.add_argument("--k", type=int, default=1024)
@@ -65,6 +66,10 @@ def main(argv=None) -> int:
                          "--compare-torch then times one launch per group instead")
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--heads", type=int, default=16)
+    ap.add_argument("--kv-heads", type=int, default=0, help="kv8_*: heads of the cache (0: --heads)")
+    ap.add_argument("--rows", type=int, default=1, help="kv8_attn: query rows of a sequence")
+    ap.add_argument("--beams", type=int, default=8)
+    ap.add_argument("--kind", default="int8", choices=["int8", "e4m3"])
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--dh", type=int, default=64)
     ap.add_argument("--attn-poly", type=int, default=None,
@@ -275,6 +280,39 @@ def main(argv=None) -> int:
         pos0 = torch.zeros(B, device=dev, dtype=torch.int32)
         fn = lambda: D.kv_write(k, v, kc, vc, pt, pos0, S, nh, dh)  # noqa: E731
         nbytes = 2.0 * 2 * 2 * B * S * nh * dh
+    elif a.kernel.startswith("kv8_"):
+        from ..ops import kv8
+        B, nkv, dh, S = a.batch, a.kv_heads or a.heads, a.dh, a.seq
+        pages = (S + kv8.PAGE - 1) // kv8.PAGE
+        cache = kv8.kv8_alloc(B * pages, nkv, dh, a.kind, dev)
+        pt = torch.randperm(B * pages, device=dev).to(torch.int32).view(B, pages)
+        zero = torch.zeros(B, device=dev, dtype=torch.int32)
+        row0 = torch.arange(B + 1, device=dev, dtype=torch.int32) * S
+        k, v = torch.randn(2, B * S, nkv * dh, device=dev, dtype=bf)
+        fill = lambda: kv8.kv8_write(k, v, *cache, pt, zero, row0, S)  # noqa: E731
+        size = B * S * nkv * dh
+        if a.kernel == "kv8_write":
+            fn, nbytes = fill, 2.0 * 3 * size
+        elif a.kernel == "kv8_read":
+            fill()
+            fn = lambda: kv8.kv8_read(*cache, pt, zero, row0, B * S, S)  # noqa: E731
+            nbytes = 2.0 * 3 * size
+        else:
+            fill()
+            q = torch.randn(B * a.rows, a.heads * dh, device=dev, dtype=bf)
+            ctx = torch.full((B,), S, device=dev, dtype=torch.int32)
+            first = torch.arange(B + 1, device=dev, dtype=torch.int32) * a.rows
+            fn = lambda: kv8.kv8_attention(q, *cache, pt, ctx, a.heads, first, a.rows)  # noqa: E731
+            nbytes = 2.0 * size + 4.0 * q.numel()
+            flops = 4.0 * q.numel() * (S - (a.rows - 1) / 2)
+    elif a.kernel == "beam_select":
+        from ..ops import beam
+        B, K, V = a.batch, a.beams, a.vocab
+        logits = torch.randn(B * K, V, device=dev).to(bf)
+        scores = -torch.rand(B, K, device=dev).sort(-1).values
+        done = torch.zeros(B, K, device=dev, dtype=torch.bool)
+        fn = lambda: beam.beam_select(logits, scores, done, None)  # noqa: E731
+        nbytes = 2.0 * B * K * V
     elif a.kernel == "argmax":
         B, V = a.batch, a.vocab
         logits = torch.randn(B, V, device=dev).to(bf)

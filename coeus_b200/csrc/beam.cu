@@ -398,9 +398,13 @@ struct CopyArgs {
   int bytes[COPY_MAX];                 // of a page, a multiple of 4
 };
 __global__ void __launch_bounds__(256) beam_copy_kernel(const __grid_constant__ CopyArgs a, const int* __restrict__ src,
-                                                        const int* __restrict__ dst) {
+                                                        const int* __restrict__ dst, int num_pages, int* status) {
   const int s = src[blockIdx.x], d = dst[blockIdx.x];
   if (s < 0 || d < 0 || s == d) return;
+  if (s >= num_pages || d >= num_pages) {
+    if (threadIdx.x == 0) record_status(status, ST_BOUNDS, blockIdx.x);
+    return;
+  }
   const size_t bytes = a.bytes[blockIdx.y];
   const char* from = static_cast<const char*>(a.base[blockIdx.y]) + s * bytes;
   char* to = static_cast<char*>(a.base[blockIdx.y]) + d * bytes;
@@ -463,7 +467,7 @@ extern "C" int cb_beam_pages(const int* table, int width, int B, int K, const in
 
 // Copies page src[i] to page dst[i] (-1: none) in every tensor; base and bytes are host arrays.
 extern "C" int cb_beam_copy(void* const* base, const int* bytes, int tensors, const int* src, const int* dst, int n,
-                            void* stream) {
+                            int num_pages, int* status, void* stream) {
   if (n < 1 || tensors < 1) return -1;
   for (int t0 = 0; t0 < tensors; t0 += COPY_MAX) {
     CopyArgs a;
@@ -475,8 +479,9 @@ extern "C" int cb_beam_copy(void* const* base, const int* bytes, int tensors, co
       if (a.bytes[t] < 4 || a.bytes[t] % 4 != 0) return -2;
       most = a.bytes[t] > most ? a.bytes[t] : most;
     }
-    const dim3 grid(n, nt, (most + 16383) / 16384);
-    beam_copy_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a, src, dst);
+    const int parts = static_cast<int>((most + 16383ll) / 16384);
+    const dim3 grid(n, nt, parts < 65535 ? parts : 65535);
+    beam_copy_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a, src, dst, num_pages, status);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

@@ -164,7 +164,8 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
 
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
     """Copies page ``src[i]`` to page ``dst[i]`` (int32, -1: nothing) in every tensor of ``caches``, whose
-    first dimension is the page.  A page that is written is neither read nor written twice."""
+    first dimension is the page.  A page that is written is neither read nor written twice.  A page that the
+    tensors do not have is not copied, and the status word says so."""
     if src.shape != dst.shape or src.dim() != 1 or src.dtype != torch.int32 \
             or dst.dtype != torch.int32:
         raise ValueError("copy_pages: src and dst are int32 of one length")
@@ -188,13 +189,16 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
         if max(sizes) >= 1 << 31:
             raise ValueError("copy_pages: a page of 2 GB or more")
         with _lib.on_device(device):
-            rc = _lib.entry("cb_beam_copy", "ppippip")(
-                (ctypes.c_void_p * n)(*base), (ctypes.c_int * n)(*sizes), n,
-                src.contiguous().data_ptr(), dst.contiguous().data_ptr(), src.numel(),
-                _lib.stream_int())
+            src, dst = src.contiguous(), dst.contiguous()
+            rc = _lib.entry("cb_beam_copy", "ppippiipp")(
+                (ctypes.c_void_p * n)(*base), (ctypes.c_int * n)(*sizes), n, src.data_ptr(),
+                dst.data_ptr(), src.numel(), pages,
+                _lib.status_buffer(src.device).data_ptr(), _lib.stream_int())
         _lib.check_rc(rc, "cb_beam_copy", launches=(n + 191) // 192)
         return
     for s, d in zip(src.tolist(), dst.tolist()):
+        if max(s, d) >= pages and min(s, d) >= 0:
+            raise ValueError(f"copy_pages: page {s} to page {d} of {pages}")
         if s >= 0 and d >= 0:
             for c in caches:
                 raw = c.view(torch.int8) if c.element_size() == 1 else c

@@ -36,6 +36,15 @@ def test_reorder(lens, K):
     check_reorder(table, parent, lens, pool, caches)       # and on from there
 
 
+def test_copies_of_pages_that_are_not_there():
+    c = torch.arange(8).view(4, 2)
+    for s, d in ((4, 1), (1, 4)):
+        with pytest.raises(ValueError):
+            beam.copy_pages([c], torch.tensor([s], dtype=torch.int32), torch.tensor([d], dtype=torch.int32))
+    beam.copy_pages([c], torch.tensor([-1, 0], dtype=torch.int32), torch.tensor([9, 1], dtype=torch.int32))
+    assert c.tolist() == [[0, 1], [0, 1], [4, 5], [6, 7]]
+
+
 def test_refusals():
     logits, scores, done = state(2, 3, 9, torch.float32, "cpu")
     for args in ((logits[:5], scores, done, 1), (logits, scores.double(), done, 1),

@@ -111,6 +111,20 @@ def test_reorder_many_tensors_and_graph():
     assert torch.equal(out, want) and status() == 0
 
 
+def test_copies_of_pages_that_are_not_there():
+    """Only the copies that the tensors have are made; the others are reported."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    caches = [torch.arange(5 * 48, device=DEV, dtype=torch.int32).view(5, 48), torch.rand(5, 7, device=DEV)]
+    before = [c.clone() for c in caches]
+    beam.copy_pages(caches, i32([0, 2, 5, 2 ** 31 - 1]), i32([1, 2 ** 31 - 1, 3, 4]))
+    assert status() == 2
+    for c, b in zip(caches, before):
+        b[1] = b[0]
+        assert torch.equal(c, b)
+    beam.copy_pages(caches, i32([-1, 3]), i32([2, -5]))
+    assert status() == 0 and all(torch.equal(c, b) for c, b in zip(caches, before))
+
+
 def test_reorder_reports_what_it_cannot_do():
     table, pool, total = pages_case(2, 3, [70, 20], 2, DEV)
     cache = [torch.arange(total * 4, device=DEV, dtype=torch.float32).view(total, 4)]

@@ -369,7 +369,13 @@ __global__ void __launch_bounds__(256) beam_pages_kernel(const int* __restrict__
     for (int i0 = 0; i0 < pool_n && n < K; i0 += 32) {
       const int i = i0 + threadIdx.x;
       const int page = i < pool_n ? pool[static_cast<size_t>(item) * pool_n + i] : -1;
-      const bool ok = page >= 0 && page < num_pages && !(used[page / 32] >> (page % 32) & 1u);
+      bool ok = page >= 0 && page < num_pages && !(used[page / 32] >> (page % 32) & 1u);
+      // a page that the pool names twice is one page
+      const uint32_t same = __match_any_sync(0xffffffffu, ok ? page : -1 - static_cast<int>(threadIdx.x));
+      ok = ok && (same & ((1u << threadIdx.x) - 1u)) == 0;
+      __syncwarp();
+      if (ok) mark(page);
+      __syncwarp();
       const uint32_t all = __ballot_sync(0xffffffffu, ok);
       const int place = n + __popc(all & ((1u << threadIdx.x) - 1u));
       if (ok && place < K) s_free[place] = page;

@@ -98,7 +98,7 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
     for the next one.  Full pages are taken over from the parent.  If the last page is not full, the
     first child of a parent keeps it and the others copy it to free pages; if it is, every beam gets a
     free page.  Free pages come from ``pool [B, n]`` (int32, the pages that belong to the request), in its
-    order, without those that a new row of the request holds; ``K`` times the pages that a beam can have
+    order and each once, without those that a new row of the request holds; ``K`` times the pages that a beam can have
     on its own, plus ``K``, always suffice.  When they do not, the row's entry is -1 and the status word
     says so.  Columns behind the next token's page keep what the row had."""
     if parent.dim() != 2 or parent.dtype != torch.int64:
@@ -147,7 +147,7 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
             held.update(page_table[b * K + p, :lp].tolist())
             if rest and p not in par[:j]:
                 held.add(int(page_table[b * K + p, lp]))
-        free = iter([p for p in pool[b].tolist() if p not in held])
+        free = iter(dict.fromkeys(p for p in pool[b].tolist() if p not in held))
         for j, p in enumerate(par):
             tail = int(page_table[b * K + p, lp])
             if rest and p not in par[:j]:

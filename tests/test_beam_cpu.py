@@ -63,3 +63,14 @@ def test_refusals():
                    (4, [cache[0].t()]), (4, [cache[0], torch.zeros(total + 1, 4)])):
         with pytest.raises(ValueError):
             beam.beam_reorder(*[bad if j == i else x for j, x in enumerate(good)])
+
+
+def test_pool_that_names_a_page_twice():
+    table, pool, total = pages_case(2, 4, [70, 20], 2, "cpu")
+    n, parent = torch.tensor([70, 20], dtype=torch.int32), torch.tensor([[0, 0, 0, 2], [1, 1, 1, 1]])
+    want, src, dst = beam.beam_pages(table, parent, n, pool, total)
+    twice = torch.cat([pool[:, :1], pool.repeat_interleave(3, 1), pool], 1)
+    got, s, d = beam.beam_pages(table, parent, n, twice, total)
+    assert torch.equal(got, want) and torch.equal(s, src) and torch.equal(d, dst)
+    for b, lp in ((0, 1), (1, 0)):
+        assert len(set(got.view(2, 4, -1)[b, :, lp].tolist())) == 4

@@ -142,3 +142,15 @@ def test_reorder_reports_what_it_cannot_do():
         beam.copy_pages([torch.zeros(4, 3, dtype=torch.int8, device=DEV)], n, n)
     with pytest.raises(ValueError):
         beam.beam_reorder(table, parent.cpu(), n, pool, cache)
+
+
+def test_pool_that_names_a_page_twice():
+    table, pool, total = pages_case(2, 4, [70, 20], 2, DEV)
+    n, parent = torch.tensor([70, 20], dtype=torch.int32, device=DEV), torch.tensor([[0, 0, 0, 2], [1, 1, 1, 1]], device=DEV)
+    want, src, dst = beam.beam_pages(table, parent, n, pool, total)
+    twice = torch.cat([pool[:, :1], pool.repeat_interleave(3, 1), pool], 1)
+    got, s, d = beam.beam_pages(table, parent, n, twice, total)
+    assert torch.equal(got, want) and torch.equal(s, src) and torch.equal(d, dst)
+    for b, lp in ((0, 1), (1, 0)):
+        assert len(set(got.view(2, 4, -1)[b, :, lp].tolist())) == 4
+    assert status() == 0

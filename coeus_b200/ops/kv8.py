@@ -102,7 +102,7 @@ def _rows(what: str, x: torch.Tensor, width: int, device: int) -> torch.Tensor:
         raise ValueError(f"{what}: the kernels take bf16 rows, got {x.dtype}")
     step = x.stride(0)
     if x.stride(1) != 1 or step % 8 or x.data_ptr() % 16 or not 0 <= step < 1 << 31:
-        x = x.contiguous()
+        x = x.clone(memory_format=torch.contiguous_format)   # contiguous() keeps an odd address
     return x
 
 
@@ -164,7 +164,7 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
               pos0: torch.Tensor, row0: Optional[torch.Tensor] = None, max_rows: int = 1) -> None:
     """Stores the rows of ``k`` / ``v`` (``[rows, heads * dh]`` views) at positions ``pos0[e]`` and on of
     each entry.  Tokens of the first page before ``pos0[e]`` are kept; what the page held from there on
-    is not counted on any more."""
+    is not counted on any more.  A page that is written belongs to one entry."""
     pages, heads, dh, n, device = _check("kv8_write", k_cache, v_cache, k_scale, v_scale,
                                          page_table, pos0, row0, max_rows)
     k = _rows("kv8_write", k, heads * dh, device)

@@ -105,3 +105,27 @@ def test_refusals():
         kv8.kv8_alloc(4, 2, 64, "fp4", "cpu")
     with pytest.raises(ValueError):
         kv8.kv8_read(k, v, ks, vs, c.table, pos, None, 2, 1)
+
+
+def test_rows_are_laid_out_for_the_kernels():
+    """Rows whose address, stride or order the kernels cannot read are copied, others are not."""
+    flat = torch.zeros(8 * 128 + 64, dtype=torch.bfloat16)
+    off = (-flat.data_ptr() // 2) % 8                      # numbers up to a multiple of 16 bytes
+    lay = lambda x: kv8._rows("rows", x, 64, 0 if x.get_device() == 0 else -1)
+
+    class OnDevice:                                        # a view that says it is on a GPU
+        def __init__(self, x):
+            self.x = x
+
+        def get_device(self):
+            return 0
+
+        def __getattr__(self, name):
+            return getattr(self.x, name)
+
+    for x, kept in ((flat[off:off + 256].view(4, 64), True), (flat[off + 1:off + 257].view(4, 64), False),
+                    (flat[off:off + 512].view(4, 128)[:, :64], True), (flat[off:off + 512].view(4, 128)[:, 4:68], False),
+                    (flat[off:off + 4 * 68].view(4, 68)[:, :64], False), (flat[off:off + 256].view(64, 4).t(), False)):
+        y = lay(OnDevice(x))
+        assert (y.data_ptr() == x.data_ptr()) == kept
+        assert y.data_ptr() % 16 == 0 and y.stride(1) == 1 and y.stride(0) % 8 == 0

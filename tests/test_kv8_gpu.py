@@ -354,3 +354,21 @@ def test_gpu_refusals():
     with pytest.raises(ValueError):
         kv8.kv8_read(*c.c, c.table.to(DEV), i32([0], DEV), i32([0, 1], DEV), 1, 1,
                      dtype=torch.float32)
+
+
+@pytest.mark.parametrize("shift", [1, 4])
+def test_rows_that_begin_anywhere(shift):
+    """Contiguous rows whose first one is not at a multiple of 16 bytes, for every input of rows."""
+    c = Case("int8", 2, 64, [70, 3], DEV)
+    flat = torch.randn(3, 2 * 128 + 8, generator=torch.Generator().manual_seed(5)).bfloat16().to(DEV)
+    k, v, q = (f[shift:shift + 256].view(2, 128) for f in flat)
+    assert k.is_contiguous() and k.data_ptr() % 16
+    pos, ctx = i32([0, 2], DEV), i32([1, 3], DEV)
+    got = []
+    for a, b, x in ((k, v, q), (k.clone(), v.clone(), q.clone())):
+        for t in c.c:
+            t.zero_()
+        kv8.kv8_write(a, b, *c.c, c.table.to(DEV), pos)
+        got.append([kv8.kv8_attention(x, *c.c, c.table.to(DEV), ctx, 2)] + [t.clone() for t in c.c])
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(*got))
+    assert status() == 0

@@ -285,8 +285,11 @@ def cmd_generate(store, rest: List[str]) -> dict:
     beams = int(_get(store, "beams") or 1)
     engine = make_engine(model, max_batch=beams, **_kv_dtype(store))
     prompt = torch.tensor(ids, device=device)[None]
+    eos = _get(store, "eos_id")
+    temperature = float(_get(store, "temperature") or 0.0)
     if beams > 1:
-        eos = _get(store, "eos_id")
+        if temperature:
+            raise SystemExit("--beams searches and --temperature samples: one of them")
         penalty = _get(store, "length_penalty")
         found, scores = engine.beam_search(prompt, beams, n,
                                            eos_id=None if eos is None else int(eos),
@@ -294,7 +297,8 @@ def cmd_generate(store, rest: List[str]) -> dict:
         res = {"prompt_ids": ids, "token_ids": found[0, 0, len(ids):].tolist(),
                "score": float(scores[0, 0])}
     else:
-        out = engine.generate(prompt, n, temperature=float(_get(store, "temperature") or 0.0))
+        out = engine.generate(prompt, n, temperature=temperature,
+                              eos_id=None if eos is None else int(eos))
         res = {"prompt_ids": ids, "token_ids": out[0, len(ids):].tolist()}
     if tok is not None:
         from .serve.server import _decoder
@@ -361,6 +365,8 @@ def cmd_serve(store) -> int:
     engine = group = None
     if world > 1 and not isinstance(model, DecoderLM):
         raise SystemExit(f"{model.cfg.architecture} models are served by one process")
+    if world > 1 and _kv_dtype(store):
+        raise SystemExit("a cache in 8 bits (--kv_dtype) is served by one process")
     if world > 1:
         import torch.distributed as dist
 

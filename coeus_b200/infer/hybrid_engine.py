@@ -50,10 +50,13 @@ class HybridEngine(InferenceEngine):
     prefill_tokens = 16384       # rows of one step when a prompt batch is cut by generate()
 
     def __init__(self, model: HybridLM, max_batch: int = 64, max_len: Optional[int] = None,
-                 use_graph: Optional[bool] = None) -> None:
+                 use_graph: Optional[bool] = None, kv_dtype: Optional[str] = None) -> None:
+        if kv_dtype is not None:
+            raise ProcessingError.unsupported(f"kv_dtype {kv_dtype!r} with this model",
+                                              "every layer's cache is laid out on its own")
         self.m = model
         self.cfg = model.cfg
-        self.kv_dtype = None         # every layer's cache is laid out on its own
+        self.kv_dtype = None
         self.max_batch = max_batch
         self.max_len = max_len or self.cfg.max_seq_len
         self.cache: Optional[PagedKVCache] = None

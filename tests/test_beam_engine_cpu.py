@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from coeus_b200.foundation.error import ProcessingError
-from coeus_b200.infer.engine import InferenceEngine
+from coeus_b200.infer.engine import InferenceEngine, make_engine
 from coeus_b200.infer.scheduler import ContinuousBatcher
 from coeus_b200.models.config import DecoderConfig
 from coeus_b200.models.decoder import DecoderLM
@@ -169,3 +169,22 @@ def test_command_line(tmp_path, capsys):
           "--kv_dtype=int8", "--device=cpu"])
     out = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
     assert len(out["token_ids"]) == 6 and math.isfinite(out["score"]) and out["score"] < 0.0
+    # one beam is the greedy continuation, which the end token ends too
+    args = ["generate", f"--weights={path}", "--prompt_ids=5,6,7", "--max_tokens=6", "--device=cpu"]
+    main(args)
+    plain = json.loads(capsys.readouterr().out.strip().splitlines()[-1])["token_ids"]
+    main(args + [f"--eos_id={plain[1]}"])
+    ended = json.loads(capsys.readouterr().out.strip().splitlines()[-1])["token_ids"]
+    first = plain.index(plain[1])
+    assert ended[:first + 1] == plain[:first + 1] and set(ended[first + 1:]) <= {plain[1]}
+    with pytest.raises(SystemExit):
+        main(args + ["--beams=2", "--temperature=0.8"])
+
+
+def test_mixed_layers_refuse_8_bits():
+    from dogilorn_cases import Bench
+    m = Bench("odd", "cpu", torch.float32).lm
+    with pytest.raises(ProcessingError):
+        make_engine(m, kv_dtype="int8")
+    with pytest.raises(ProcessingError):
+        make_engine(m).beam_search(torch.zeros((1, 3), dtype=torch.int64), 2, 3)

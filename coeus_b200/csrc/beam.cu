@@ -12,9 +12,10 @@
 //          another block.  So the blocks' maxima choose K blocks, and only those are read again.
 //
 // Pages.  A request's beams share the pages of what they have in common.  With n tokens stored the next
-// one goes to page n / 64: full pages are taken over from the parent by number; of the children of
-// one parent the first keeps its page of n mod 64 tokens, the others get a free page of the request's pool
-// and a copy.  A page is free when no new row of the request holds it, so nothing is counted from step to step.
+// one goes to page n / 64: full pages are taken over from the parent by number; of the beams whose parents
+// hold the same page of n mod 64 tokens (children of one parent, or of parents that have not parted yet) the first keeps
+// it, the others get a free page of the request's pool and a copy.  A page is free when no new row of the request holds
+// it, so nothing is counted from step to step.
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(256) beam_pages_kernel(const int* __restrict__
                                                          int pool_n, int num_pages, int* __restrict__ out,
                                                          int* __restrict__ src, int* __restrict__ dst, int* status) {
   extern __shared__ uint32_t used[];
-  __shared__ int s_parent[BEAM_MAX], s_keeps[BEAM_MAX], s_free[BEAM_MAX], s_turn[BEAM_MAX];
+  __shared__ int s_parent[BEAM_MAX], s_tail[BEAM_MAX], s_keeps[BEAM_MAX], s_free[BEAM_MAX], s_turn[BEAM_MAX];
   const int item = blockIdx.x, row0 = item * K;
   const int len = length[item], lp = len / BEAM_PAGE;
   const bool partial = len % BEAM_PAGE != 0;
@@ -333,11 +334,12 @@ __global__ void __launch_bounds__(256) beam_pages_kernel(const int* __restrict__
       p = threadIdx.x;
     }
     s_parent[threadIdx.x] = static_cast<int>(p);
+    s_tail[threadIdx.x] = table[static_cast<size_t>(row0 + p) * width + lp];
   }
   __syncthreads();
   if (threadIdx.x < K) {
     bool keeps = partial;
-    for (int j = 0; j < threadIdx.x; ++j) keeps = keeps && s_parent[j] != s_parent[threadIdx.x];
+    for (int j = 0; j < threadIdx.x; ++j) keeps = keeps && s_tail[j] != s_tail[threadIdx.x];
     s_keeps[threadIdx.x] = keeps;
   }
   __syncthreads();
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(256) beam_pages_kernel(const int* __restrict__
     if (!s_keeps[j]) {
       d = s_free[s_turn[j]];
       out[static_cast<size_t>(row0 + j) * width + lp] = d;
-      if (partial) s = table[static_cast<size_t>(row0 + s_parent[j]) * width + lp];
+      if (partial) s = s_tail[j];
       if (d < 0) record_status(status, ST_BOUNDS, item);       // the pool is too small
     }
     const bool copy = s >= 0 && s < num_pages && d >= 0;

@@ -96,11 +96,12 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
 
     A request's beams all hold ``length[b]`` tokens (int32); afterwards every beam has a page of its own
     for the next one.  Full pages are taken over from the parent.  If the last page is not full, the
-    first child of a parent keeps it and the others copy it to free pages; if it is, every beam gets a
-    free page.  Free pages come from ``pool [B, n]`` (int32, the pages that belong to the request), in its
-    order and each once, without those that a new row of the request holds; ``K`` times the pages that a beam can have
-    on its own, plus ``K``, always suffice.  When they do not, the row's entry is -1 and the status word
-    says so.  Columns behind the next token's page keep what the row had."""
+    first of the beams whose parents hold it (one parent, or several that share it still) keeps it and
+    the others copy it to free pages; if it is, every beam gets a free page.  Free pages come from
+    ``pool [B, n]`` (int32, the pages that belong to the request), in its order and each once, without
+    those that a new row of the request holds; ``K`` times the pages that a beam can have on its own, plus
+    ``K``, always suffice.  When they do not, the row's entry is -1 and the status word says so.  Columns
+    behind the next token's page keep what the row had."""
     if parent.dim() != 2 or parent.dtype != torch.int64:
         raise ValueError(f"beam_pages: parent is int64 [B, K], got {tuple(parent.shape)} {parent.dtype}")
     B, K = parent.shape
@@ -142,15 +143,16 @@ def beam_pages(page_table: torch.Tensor, parent: torch.Tensor, length: torch.Ten
         if n < 0 or lp >= width or any(not 0 <= p < K for p in par):
             raise ValueError(f"beam_pages: request {b} has {n} tokens, parents {par}, {width} pages")
         held = set()
+        tails = [int(page_table[b * K + p, lp]) for p in par]
+        keeps = [bool(rest) and t not in tails[:j] for j, t in enumerate(tails)]
         for j, p in enumerate(par):
             table[b * K + j, :lp] = page_table[b * K + p, :lp]
             held.update(page_table[b * K + p, :lp].tolist())
-            if rest and p not in par[:j]:
-                held.add(int(page_table[b * K + p, lp]))
+            if keeps[j]:
+                held.add(tails[j])
         free = iter(dict.fromkeys(p for p in pool[b].tolist() if p not in held))
-        for j, p in enumerate(par):
-            tail = int(page_table[b * K + p, lp])
-            if rest and p not in par[:j]:
+        for j, tail in enumerate(tails):
+            if keeps[j]:
                 table[b * K + j, lp] = tail
                 continue
             page = next(free, None)

@@ -188,3 +188,18 @@ def test_mixed_layers_refuse_8_bits():
         make_engine(m, kv_dtype="int8")
     with pytest.raises(ProcessingError):
         make_engine(m).beam_search(torch.zeros((1, 3), dtype=torch.int64), 2, 3)
+
+
+@pytest.mark.parametrize("V,K", [(3, 4), (5, 8), (7, 8), (2, 3)])
+@pytest.mark.parametrize("S", [10, 63, 64])
+def test_fewer_tokens_than_beams(V, K, S):
+    """The first steps leave places of the beam empty; those beams' rows still name the prompt's last page."""
+    for seed in range(3):
+        m = model("gpt", vocab=V, seed=seed)
+        ids = torch.randint(0, V, (1, S), generator=torch.Generator().manual_seed(seed))
+        for eos in (None, 1):
+            out, scores = InferenceEngine(m, max_batch=8).beam_search(ids, K, 5, eos_id=eos, keep=K)
+            want = plain_beams(m, ids[0].tolist(), K, 5, eos, 1.0)
+            for i, (score, tokens) in enumerate(want):
+                assert abs(float(scores[0, i]) - score) < 1e-4
+                assert out[0, i, S:].tolist() == tokens

@@ -90,3 +90,23 @@ def test_batcher(kv):
     r = b.submit(prompts[2], 9)
     assert len(b.run()[r]) == 9 and b.prefix.hits == 1
     assert status() == 0
+
+
+@pytest.mark.parametrize("kv", [None, "int8"])
+def test_fewer_tokens_than_beams(kv):
+    """The first step leaves places of the beam empty; scores are what the whole model says of the sequences, within
+    the bounds of test_beam_search."""
+    torch.manual_seed(0)
+    m = DecoderLM(DecoderConfig(hidden_dim=256, num_layers=2, num_heads=4, intermediate_dim=512, vocab_size=3,
+                                max_seq_len=256, use_bias=False, activation="swiglu", norm="rmsnorm", pos="rope"),
+                  device=DEV, training=False)
+    for S in (10, 64, 70):
+        ids = torch.randint(0, 3, (2, S), generator=torch.Generator().manual_seed(S)).to(DEV)
+        for graph in (True, False):
+            out, scores = InferenceEngine(m, max_batch=16, use_graph=graph, kv_dtype=kv).beam_search(ids, 8, 6, keep=8)
+            x = m.forward_logits(out.reshape(16, -1)[:, :-1])[..., :3].float()
+            lp = torch.log_softmax(x.view(16, -1, 3), -1)[:, S - 1:]
+            want = torch.gather(lp, 2, out.reshape(16, -1)[:, S:, None])[..., 0].sum(-1).view(2, 8) / 6
+            assert float((want - scores).abs().max()) < (0.04 if kv is None else 0.08)
+            assert all(len({tuple(x) for x in out[b].tolist()}) == 8 for b in range(2))
+    assert status() == 0

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from beam_cases import check_reorder, check_select, pages_case, state
+from beam_tails import TAILS, check_shared_tails
 from coeus_b200.ops import _lib, beam
 
 pytestmark = pytest.mark.gpu
@@ -153,4 +154,11 @@ def test_pool_that_names_a_page_twice():
     assert torch.equal(got, want) and torch.equal(s, src) and torch.equal(d, dst)
     for b, lp in ((0, 1), (1, 0)):
         assert len(set(got.view(2, 4, -1)[b, :, lp].tolist())) == 4
+    assert status() == 0
+
+
+@pytest.mark.parametrize("length", [1, 70, 191])
+@pytest.mark.parametrize("rows,parent", TAILS)
+def test_reorder_shared_tails(length, rows, parent):
+    check_shared_tails(DEV, length, rows, parent)
     assert status() == 0

@@ -202,6 +202,7 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                 if lo:
                     bad = bad | torch.isnan(scale[page])
                     was = torch.frexp(torch.nan_to_num(scale[page], 1.0))[1] - 1
+                    was = was.masked_fill(scale[page] == 0, -127)          # nothing written there yet
                     ex = torch.maximum(ex, was)
                     shift = torch.where(bad, torch.zeros_like(ex), was - ex)
                     kept = torch.ldexp(old[:, :lo], shift[:, None, None])

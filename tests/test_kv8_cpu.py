@@ -129,3 +129,30 @@ def test_rows_are_laid_out_for_the_kernels():
         y = lay(OnDevice(x))
         assert (y.data_ptr() == x.data_ptr()) == kept
         assert y.data_ptr() % 16 == 0 and y.stride(1) == 1 and y.stride(0) % 8 == 0
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("size", [1e-30, 0.03, 50.0])
+def test_first_token_inside_a_page_that_nothing_has_written(kind, size):
+    """Nothing is kept of such a page, its scale neither."""
+    DEV = "cpu"
+    c = kv8.kv8_alloc(2, 2, 64, kind, DEV)
+    k = torch.randn(3, 128, generator=torch.Generator().manual_seed(1)).mul(size).bfloat16()
+    qmax = {"int8": 127.0, "e4m3": 448.0}[kind]
+    for page, row0, pos in ((0, None, [5]), (1, i32([0, 3], DEV), [64 + 9])):
+        n = 1 if row0 is None else 3
+        kv8.kv8_write(k[:n].to(DEV), 3 * k[:n].to(DEV), *c, i32([[0, 1]], DEV), i32(pos, DEV), row0, n)
+        for x, scale in ((k[:n], c[2]), (3 * k[:n], c[3])):
+            for h in range(2):
+                top = float(x[:, 64 * h:64 * h + 64].abs().max())
+                e = max(-126, math.ceil(math.log2(top / qmax)))
+                assert float(scale[page, h]) == 2.0 ** e, (page, h, float(scale[page, h]), e)
+        got = kv8.kv8_read(*c, i32([[0, 1]], DEV), i32(pos, DEV), i32([0, n], DEV), n, n)
+        for x, y in zip((k[:n], 3 * k[:n]), got):
+            # one rounding: half a step, 2^(e - 1), is below the largest / 127; of e4m3 half of three bits, or 2^-10 of the
+            # scale for its smallest codes, which is below 2^-17 of the largest
+            top = x.abs().max().float()
+            step = top / 127.0 if kind == "int8" else x.float().abs() * 2.0 ** -4 + top * 2.0 ** -17
+            assert ((y.float().cpu() - x.float()).abs() <= step + 2.0 ** -133).all()
+        if row0 is not None:                               # what lies in front of the first token is zero
+            assert all((t == 0).all() for t in kv8.kv8_read(*c, i32([[0, 1]], DEV), i32([64], DEV), i32([0, 9], DEV), 9, 9))

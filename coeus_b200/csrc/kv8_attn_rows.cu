@@ -10,8 +10,9 @@
 //                 reads them; the running maximum, the sum, and at the end the tile's rows
 //
 // The scale 2^ev of a page's values goes into the weights: with z = s + ev (s the score in units of log2) and m a
-// running maximum of z, the weights are P = 2^(z - m), and the denominator sums 2^(e0 - ev) P, e0 the first page's ev:
-// o = 2^e0 sum P code / sum 2^(e0 - ev) P.  So pages of any scales add up in one accumulator.  The maximum is only
+// running maximum of z, the weights are P = 2^(z - m).  The denominator has a maximum of its own, md of s alone, and sums
+// 2^(m - ev - md) P = 2^(s - md): o = 2^(m - md) sum P code / sum 2^(s - md).  So pages of any scales add up in one
+// accumulator, and a page without values, whose ev says nothing, counts for the denominator alone.  m is only
 // raised when z exceeds it by more than KB_LAG, and the sums so far are multiplied then.  A page of a tile is 2 x 64 x 128 dh
 // multiply-adds and 8192 exponentials; what bounds it is the chain of score product, softmax and value product, two tiles
 // an SM in turn.  Four sequences of 8192 with 512 rows each, 32 heads over 8 of 128: 448 us and 18 for the merge, 0.35 of
@@ -30,6 +31,7 @@ constexpr int KB_PLACES = 2;                      // CTAs that share an SM: the 
 // Weights are held times 2^KB_SHIFT and are at most 2^(KB_SHIFT + KB_LAG) < 65504; fp16 keeps their digits down to 2^-24
 // of the row's largest, and 2^-34 is lost.
 constexpr float KB_SHIFT = 10.f, KB_LAG = 4.f;
+constexpr float KB_LOST = 36.f;                   // weights up to 2^(KB_SHIFT - KB_LOST) are zero in fp16
 constexpr uint32_t KB_O = 0, KB_S = 128, KB_COLS = 256;                  // columns of tensor memory; weights lie on their scores
 
 template <int DH>
@@ -331,8 +333,8 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
       const int rows = t.w.x.rows, ctx = t.w.x.ctx, total = rows * a.group, rr = t.w.tile * KB_ROWS + tid;
       const int seen = ctx - rows + min(rr, total - 1) / a.group + 1;
       const int least_seen = ctx - rows + t.w.tile * KB_ROWS / a.group + 1;
-      float m = -INFINITY, l = 0.f, f = 0.f;
-      int e0 = 0, e_top = -1000;                                 // the first page's scale, the largest so far
+      float m = -INFINITY, md = -INFINITY, l = 0.f, f = 0.f;     // maxima of z and s, sum of 2^(s - md)
+      int e_top = -1000;                                         // the largest scale so far
       for (int p = t.p0; p < t.p1; ++p, ++gi) {
         const int st = gi % KB_STAGES, base = p * KV8_PAGE;
         wait(full + st, gi / KB_STAGES);
@@ -342,17 +344,13 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
         if (p == t.p0) f = sf[(tiles & 3) * KB_ROWS + tid];
         const float4 mt = meta[st];
         const uint32_t sa = mine + KB_S + (gi & 1) * KV8_PAGE;
-        // A page without values (the smallest scale there is) has weights for the denominator only, under whatever scale;
-        // one whose values are next to nothing against another's counts as if they were 2^-40 of these.
-        const bool fine = mt.y == mt.y, none = fine && mt.y <= 1.17549435e-38f;
+        // One whose values are next to nothing against another's counts as if they were 2^-40 of these.
+        const bool fine = mt.y == mt.y;
         int ev = fine ? (__float_as_int(mt.y) >> 23) - 127 : 0;
-        if (fine && !none) {
+        if (fine) {
           e_top = max(e_top, ev);
           ev = max(ev, e_top - 40);
-        } else {
-          ev = e_top > -1000 ? e_top : 0;
         }
-        if (p == t.p0) e0 = ev;
         const float fk = f * mt.x, ef = fine ? static_cast<float>(ev) : mt.y;
         const bool whole = base + KV8_PAGE <= least_seen && mt.z != 0.f;
         const int n_seen = mt.z != 0.f ? seen - base : 0;        // keys of the page that the row sees
@@ -373,13 +371,12 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
 #pragma unroll
             for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
         }
-        const float z = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fk, ef);       // NaN: no maximum
+        const float smax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fk, z = smax + ef;      // NaN: no maximum
         const bool raise = z > m + KB_LAG || (m == -INFINITY && z > -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = raise ? z : m;
           const float c = mn == m ? 1.f : fast_exp2(m - mn);
           m = mn;
-          l *= c;
           if (p > t.p0) {                                        // the sums so far: the last product is over
             wait(o_done + ((gi - 1) & 1), (gi - 1) >> 1);
             tc_fence_after();
@@ -396,7 +393,11 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
             tmem_st_wait();
           }
         }
-        const float sub = KB_SHIFT + ef - (m == -INFINITY ? 0.f : m);
+        // Weights below what fp16 holds (m so far above z) are for the denominator only, and formed for it.
+        const bool lost = z + KB_LOST < m || mt.y == 0.f;
+        const float mdn = n_seen > 0 && smax > md ? smax : md, m0 = m == -INFINITY ? 0.f : m, md0 = mdn == -INFINITY ? 0.f : mdn;
+        const float sub = KB_SHIFT + (lost ? -md0 : ef - m0);
+        const float unit = fast_exp2((lost ? 0.f : m0 - static_cast<float>(ev) - md0) - KB_SHIFT);
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -421,10 +422,11 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
             add2(sum[2], sum[3], sum[2], sum[3], s[i + 2], s[i + 3]);
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = none ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
+          for (int i = 0; i < 16; ++i) w[i] = lost ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
           tmem_st_32x32b_x16(sa + 16 * h, w);                    // on scores that have been read
         }
-        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(max(min(e0 - ev, 100), -126)), l);
+        if (n_seen > 0) l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), unit, md == mdn ? l : l * fast_exp2(md - mdn));
+        md = mdn;
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(p_full + (gi & 1)));
@@ -439,7 +441,10 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
         if (dead) break;
         tc_fence_after();
       }
-      const float up = pow2(max(e0, -126)), inv = seen > 0 && summed ? up / l : 0.f;
+      // 2^(m - md) in two factors, so that none leaves fp32's range before the product does
+      constexpr float down = 1.f / (1 << static_cast<int>(KB_SHIFT));
+      const float up = md > -INFINITY ? fast_exp2(0.5f * (m - md)) : 1.f, inv = seen > 0 && summed ? up / l : 0.f;
+      auto part = [&](uint32_t x) { return __uint_as_float(x) * down * up * up; };
       __nv_bfloat16* dst = a.out + static_cast<size_t>(t.w.x.first + rr / a.group) * a.ldo + (t.w.hk * a.group + rr % a.group) * DH;
 #pragma unroll
       for (int i = 0; i < DH; i += 32) {
@@ -457,19 +462,19 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
             for (int j = 0; j < 32; j += 8) {
               float v[8];
 #pragma unroll
-              for (int x = 0; x < 8; ++x) v[x] = seen > 0 ? __uint_as_float(o[j + x]) * inv : 0.f;
+              for (int x = 0; x < 8; ++x) v[x] = seen > 0 ? __uint_as_float(o[j + x]) * down * up * inv : 0.f;
               store8(dst + i + j, v);
             }
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
               *reinterpret_cast<uint4*>(a.part_o + (slot * KB_ROWS + tid) * DH + i + j) = 
-                  make_uint4(__float_as_uint(__uint_as_float(o[j]) * up), __float_as_uint(__uint_as_float(o[j + 1]) * up),
-                             __float_as_uint(__uint_as_float(o[j + 2]) * up), __float_as_uint(__uint_as_float(o[j + 3]) * up));
+                  make_uint4(__float_as_uint(part(o[j])), __float_as_uint(part(o[j + 1])),
+                             __float_as_uint(part(o[j + 2])), __float_as_uint(part(o[j + 3])));
           }
         }
       }
-      if (!t.whole && rr < total) *reinterpret_cast<float2*>(a.part_ml + (slot * KB_ROWS + tid) * 2) = make_float2(m - static_cast<float>(e0), l);
+      if (!t.whole && rr < total) *reinterpret_cast<float2*>(a.part_ml + (slot * KB_ROWS + tid) * 2) = make_float2(md, l);
       tc_fence_before();
     }
   }

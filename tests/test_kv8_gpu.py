@@ -399,3 +399,29 @@ def test_first_token_inside_a_page_that_nothing_has_written(kind, size):
         if row0 is not None:                               # what lies in front of the first token is zero
             assert all((t == 0).all() for t in kv8.kv8_read(*c, i32([[0, 1]], DEV), i32([64], DEV), i32([0, 9], DEV), 9, 9))
     assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("size", [0.3, 1e-5, 1e-6, 1e-20, 1e-36])
+def test_wide_tiles_pages_without_values(kind, dh, size):
+    """Pages without values, or never written, count for the denominator and for nothing else, wherever they lie and
+    however small the other pages' values are."""
+    for empty in (0, 1, 3):
+        c = Case(kind, 1, dh, [400], DEV)
+
+        def edit(k, v):
+            k[:] = k.float().mul(0.5).bfloat16()
+            v[:] = v.float().mul(size).bfloat16()
+            k[64 * empty:64 * empty + 64] = 1.0            # most rows listen to it more than to the others
+            v[64 * empty:64 * empty + 64] = 0.0
+        c.write([0], [400], edit=edit)
+        q = (torch.randn(90, 2 * dh, generator=c.gen) + 0.25).bfloat16()
+        got = c.attend(q, [400], [90], 2).double().cpu()
+        want, spread = c.plain.attention(q, c.table, [400], [90], 2, dh ** -0.5)
+        # as in check_attend, and what bf16 holds of numbers next to its smallest
+        assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * spread + 2.0 ** -133).all()
+    c = Case(kind, 1, dh, [400], DEV)
+    c.write([64], [336], sizes=[size])
+    c.check_attend([400], [90], 2)
+    assert status() == 0

@@ -12,8 +12,10 @@
 // The scale 2^ev of a page's values goes into the weights: with z = s + ev (s the score in units of log2) and m a
 // running maximum of z, the weights are P = 2^(z - m).  The denominator has a maximum of its own, md of s alone, and sums
 // 2^(m - ev - md) P = 2^(s - md): o = 2^(m - md) sum P code / sum 2^(s - md).  So pages of any scales add up in one
-// accumulator, and a page without values, whose ev says nothing, counts for the denominator alone.  m is only
-// raised when z exceeds it by more than KB_LAG, and the sums so far are multiplied then.  A page of a tile is 2 x 64 x 128 dh
+// accumulator, and a page without values, whose ev says nothing, counts for the denominator alone.  m and md are whole
+// numbers, only raised when they are exceeded by more than KB_LAG, and the sums so far are multiplied then.  Where a page's
+// scale is far below that of the sums (KB_NEAR) but its scores are not, m is lowered to md + ev: its values may be all that
+// some channels have.  A page of a tile is 2 x 64 x 128 dh
 // multiply-adds and 8192 exponentials; what bounds it is the chain of score product, softmax and value product, two tiles
 // an SM in turn.  Four sequences of 8192 with 512 rows each, 32 heads over 8 of 128: 448 us and 18 for the merge, 0.35 of
 // the bf16 rate.  Four of 2000 to 8200 with 301 to 700 rows: 351 us in all, 469 with one CTA an SM and one issuing thread;
@@ -28,10 +30,14 @@ constexpr int KB_SHARE = 4;                       // pages a CTA takes at least
 constexpr int KB_THREADS = 320;
 constexpr int KB_STAGES = 2;
 constexpr int KB_PLACES = 2;                      // CTAs that share an SM: the waits of one are the other's time
-// Weights are held times 2^KB_SHIFT and are at most 2^(KB_SHIFT + KB_LAG) < 65504; fp16 keeps their digits down to 2^-24
+// Weights are held times 2^KB_SHIFT and are at most 2^(KB_SHIFT + KB_LAG) < 65504; fp16 keeps their digits down to 2^-23
 // of the row's largest, and 2^-34 is lost.
 constexpr float KB_SHIFT = 10.f, KB_LAG = 4.f;
 constexpr float KB_LOST = 36.f;                   // weights up to 2^(KB_SHIFT - KB_LOST) are zero in fp16
+// Scales that lie under those of the sums by this much lower m, and by how much at most in all: 2^20 keys, weights of 2^14
+// and codes of 2^9 leave fp32 that room.
+constexpr float KB_NEAR = 8.f, KB_DEEP = 70.f;
+constexpr float KB_NONE = -1e30f;                 // maxima of rows that have seen nothing
 constexpr uint32_t KB_O = 0, KB_S = 128, KB_COLS = 256;                  // columns of tensor memory; weights lie on their scores
 
 template <int DH>
@@ -333,8 +339,8 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
       const int rows = t.w.x.rows, ctx = t.w.x.ctx, total = rows * a.group, rr = t.w.tile * KB_ROWS + tid;
       const int seen = ctx - rows + min(rr, total - 1) / a.group + 1;
       const int least_seen = ctx - rows + t.w.tile * KB_ROWS / a.group + 1;
-      float m = -INFINITY, md = -INFINITY, l = 0.f, f = 0.f;     // maxima of z and s, sum of 2^(s - md)
-      int e_top = -1000;                                         // the largest scale so far
+      float m = KB_NONE, md = KB_NONE, l = 0.f, f = 0.f;         // maxima of z and s, sum of 2^(s - md)
+      float m_top = KB_NONE;                                     // the largest m so far
       for (int p = t.p0; p < t.p1; ++p, ++gi) {
         const int st = gi % KB_STAGES, base = p * KV8_PAGE;
         wait(full + st, gi / KB_STAGES);
@@ -344,14 +350,8 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
         if (p == t.p0) f = sf[(tiles & 3) * KB_ROWS + tid];
         const float4 mt = meta[st];
         const uint32_t sa = mine + KB_S + (gi & 1) * KV8_PAGE;
-        // One whose values are next to nothing against another's counts as if they were 2^-40 of these.
-        const bool fine = mt.y == mt.y;
-        int ev = fine ? (__float_as_int(mt.y) >> 23) - 127 : 0;
-        if (fine) {
-          e_top = max(e_top, ev);
-          ev = max(ev, e_top - 40);
-        }
-        const float fk = f * mt.x, ef = fine ? static_cast<float>(ev) : mt.y;
+        const float ev = mt.y == mt.y ? static_cast<float>((__float_as_int(mt.y) >> 23) - 127) : 0.f;
+        const float fk = f * mt.x, ef = mt.y == mt.y ? ev : mt.y;
         const bool whole = base + KV8_PAGE <= least_seen && mt.z != 0.f;
         const int n_seen = mt.z != 0.f ? seen - base : 0;        // keys of the page that the row sees
         // The row's scores twice, 32 at a time (two CTAs leave a thread 96 registers): for the maximum, then for the weights.
@@ -372,12 +372,21 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
             for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
         }
         const float smax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fk, z = smax + ef;      // NaN: no maximum
-        const bool raise = z > m + KB_LAG || (m == -INFINITY && z > -INFINITY);
-        if (__any_sync(0xffffffffu, raise)) {
-          const float mn = raise ? z : m;
-          const float c = mn == m ? 1.f : fast_exp2(m - mn);
+        float scale_gap = m - md - ev;                           // of the sums over the page
+        const bool over = z > m + KB_LAG || smax > md + KB_LAG, under = scale_gap > KB_NEAR && mt.y > 1.17549435e-38f;
+        if (__any_sync(0xffffffffu, over || under)) {
+          if (smax > md + KB_LAG) {
+            const float mdn = ceilf(smax);
+            l *= fast_exp2(md - mdn);
+            md = mdn;
+          }
+          const bool lower = under && z + KB_LOST > md + ev && m_top - m < KB_DEEP;
+          const float mn = z > m + KB_LAG ? ceilf(z) : lower ? fmaxf(fmaxf(md + ev, ceilf(z)), m_top - KB_DEEP) : m;
+          m_top = fmaxf(m_top, mn);
+          const float c = mn == m ? 1.f : fast_exp2(m - mn);     // exact
           m = mn;
-          if (p > t.p0) {                                        // the sums so far: the last product is over
+          scale_gap = m - md - ev;
+          if (p > t.p0 && __any_sync(0xffffffffu, c != 1.f)) {   // the sums so far: the last product is over
             wait(o_done + ((gi - 1) & 1), (gi - 1) >> 1);
             tc_fence_after();
 #pragma unroll
@@ -395,9 +404,8 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
         }
         // Weights below what fp16 holds (m so far above z) are for the denominator only, and formed for it.
         const bool lost = z + KB_LOST < m || mt.y == 0.f;
-        const float mdn = n_seen > 0 && smax > md ? smax : md, m0 = m == -INFINITY ? 0.f : m, md0 = mdn == -INFINITY ? 0.f : mdn;
-        const float sub = KB_SHIFT + (lost ? -md0 : ef - m0);
-        const float unit = fast_exp2((lost ? 0.f : m0 - static_cast<float>(ev) - md0) - KB_SHIFT);
+        const float sub = KB_SHIFT + (lost ? -md : ef - m);
+        const float unit = fast_exp2((lost ? 0.f : scale_gap) - KB_SHIFT);
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -425,8 +433,7 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
           for (int i = 0; i < 16; ++i) w[i] = lost ? 0u : half2_bits(s[2 * i], s[2 * i + 1]);
           tmem_st_32x32b_x16(sa + 16 * h, w);                    // on scores that have been read
         }
-        if (n_seen > 0) l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), unit, md == mdn ? l : l * fast_exp2(md - mdn));
-        md = mdn;
+        if (n_seen > 0) l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), unit, l);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(p_full + (gi & 1)));
@@ -443,7 +450,7 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
       }
       // 2^(m - md) in two factors, so that none leaves fp32's range before the product does
       constexpr float down = 1.f / (1 << static_cast<int>(KB_SHIFT));
-      const float up = md > -INFINITY ? fast_exp2(0.5f * (m - md)) : 1.f, inv = seen > 0 && summed ? up / l : 0.f;
+      const float up = md > KB_NONE ? fast_exp2(0.5f * (m - md)) : 1.f, inv = seen > 0 && summed ? up / l : 0.f;
       auto part = [&](uint32_t x) { return __uint_as_float(x) * down * up * up; };
       __nv_bfloat16* dst = a.out + static_cast<size_t>(t.w.x.first + rr / a.group) * a.ldo + (t.w.hk * a.group + rr % a.group) * DH;
 #pragma unroll
@@ -474,7 +481,7 @@ __global__ void __launch_bounds__(KB_THREADS, KB_PLACES) kv8_rows_kernel(const _
           }
         }
       }
-      if (!t.whole && rr < total) *reinterpret_cast<float2*>(a.part_ml + (slot * KB_ROWS + tid) * 2) = make_float2(md, l);
+      if (!t.whole && rr < total) *reinterpret_cast<float2*>(a.part_ml + (slot * KB_ROWS + tid) * 2) = make_float2(md > KB_NONE ? md : -INFINITY, l);
       tc_fence_before();
     }
   }

@@ -425,3 +425,62 @@ def test_wide_tiles_pages_without_values(kind, dh, size):
     c.write([64], [336], sizes=[size])
     c.check_attend([400], [90], 2)
     assert status() == 0
+
+
+def apart(c, low, high, pages, sparse=False):
+    """Keys that tell two kinds of pages apart, and values of either kind: ``pages`` says which kind."""
+    n = 64 * len(pages)
+
+    def edit(k, v):
+        for i, big in enumerate(pages):
+            at = slice(64 * i, 64 * i + 64)
+            k[at] = -1.0 if big else 1.0
+            v[at] = v[at].float().mul(2.0 ** (high if big else low)).bfloat16()
+            if big and sparse:
+                v[at, ::2] = 0.0
+    c.write([0], [n], edit=edit)
+
+
+def check_apart(c, n, rows, dh, gap, size=1.0):
+    """Rows whose scores of the two kinds of pages are ``gap`` units of log2 apart (the small values' ones above)."""
+    q = torch.full((rows, dh), gap * math.log(2.0) / (2 * dh ** 0.5))
+    q[1::2] *= torch.rand(rows // 2, 1, generator=c.gen)
+    q = (q * size).bfloat16()
+    got = c.attend(q, [n], [rows], 1).double().cpu()
+    want, spread = c.plain.attention(q, c.table, [n], [rows], 1, dh ** -0.5)
+    # as in check_attend: scores stay below 2^8 here too.  And what the fp16 weights of a wide tile cannot hold beside the
+    # row's largest product of weight and scale: they are 2^10 times what they count against a maximum up to 2^70 under that
+    # one's, less than 2^-25 is lost, and a code is below 2^9: 2^(9 - 25 - 10 - 70) of it per key, of less than 2^13 keys.  The
+    # largest one's key has a code of one or more in some channel, so the row's largest sum is no smaller than that product.
+    deep = 2.0 ** -83 * spread.view(rows, -1).amax(1, keepdim=True)
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * spread + deep + 2.0 ** -133
+    bad = (got - want).abs() > bound
+    assert not bad.any(), float(((got - want).abs() / bound)[bad].max())
+
+
+ORDERS = [[1, 0, 0, 0], [0, 1, 0, 0], [1, 1, 0, 1, 0, 0, 1, 0], [0, 0, 0, 1]]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("low,high", [(-30, 20), (-36, 14), (-60, 40), (-110, 100)])
+def test_wide_tiles_values_apart(kind, dh, low, high):
+    """Rows that listen to one kind of page alone, and to both, however far apart the values' scales are."""
+    for pages in ORDERS + [[1] + [0, 0, 1] * 30]:
+        c = Case(kind, 1, dh, [64 * len(pages)], DEV)
+        apart(c, low, high, pages)
+        for gap in (0.0, 20.0, 90.0, 120.0):
+            check_apart(c, 64 * len(pages), 100, dh, gap)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [1, 5, 100])
+def test_values_apart_channel_by_channel(kind, rows):
+    """Channels that the large values leave free hold the small ones."""
+    for pages in ORDERS:
+        c = Case(kind, 1, 128, [64 * len(pages)], DEV)
+        apart(c, -25, 20, pages, sparse=True)
+        for gap in (0.0, 15.0, -15.0):
+            check_apart(c, 64 * len(pages), rows, 128, gap)
+    assert status() == 0

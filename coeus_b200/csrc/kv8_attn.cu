@@ -24,8 +24,9 @@
 //            word s of its 16 bytes of a row of values
 // Codes become fp16 exactly: int8 by setting the biased byte into the mantissa of 1024 and subtracting, e4m3
 // by its conversion.  Queries are fp16 after division by a power of two per row.  Weights enter the second product
-// as fp16 times 2^12: smaller than 2^-26 of the row's largest they start to lose bits, and less than 2^-36
-// of it is lost in all; the page's 2^ev is applied in fp32 to the sums of a page.
+// as fp16 times 2^12, against the largest of their page: smaller than 2^-26 of it they start to lose bits, and less than
+// 2^-36 of it is lost in all.  What a page's largest weight is against the row's, and the page's 2^ev, are applied in fp32 to
+// the sums of the page, so that a page of little weight keeps its part however large its values are.
 #include "kv8_attn.cuh"
 
 namespace cb {
@@ -43,7 +44,7 @@ constexpr int KA_NARROW = 24, KA_WIDE = 64, KA_WORK = 7000;
 constexpr int KA_BLOCK = 16;                      // units that are planned at a time
 constexpr int KA_RING = 4;                        // copies in a warp's ring: the keys and values of two pages
 constexpr int KA_PLACES = 6, KA_PLACES64 = 11;    // CTAs that share an SM, by its shared memory: dh 128, 64
-constexpr float KA_SHIFT = 12.f;                  // weights are held times 2^12
+constexpr float KA_SHIFT = 12.f;                  // weights are held times 2^12 against their page's largest
 
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
           for (int x = 0; x < 4; ++x)
             if (key0 + 4 * y + 2 * (x >> 1) >= seen[x & 1]) s[y][x] = -INFINITY;
       }
-      float sub[2], fk[2];
+      float sub[2], fk[2], part[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float mx = max3(fmaxf(s[0][i], s[0][2 + i]), fmaxf(s[1][i], s[1][2 + i]), max3(s[2][i], s[2][2 + i], fmaxf(s[3][i], s[3][2 + i])));
@@ -300,12 +301,14 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         fk[i] = f[i] * ks;
-        const float mn = fmaxf(m[i], mx * fk[i]);
+        const bool sees = base < seen[i];                        // a row that sees none of it takes none, NaN neither
+        const float mp = sees ? mx * fk[i] : -INFINITY, mn = fmaxf(m[i], mp);
         const float base_m = mn == -INFINITY ? 0.f : mn;
         keep[i] = fast_exp2(m[i] - base_m);
         m[i] = mn;
-        sub[i] = KA_SHIFT - base_m;
-        scale_v[i] = base < seen[i] ? vs : 0.f;                  // a row that sees none of it takes none, NaN neither
+        sub[i] = KA_SHIFT - (mp == -INFINITY ? 0.f : mp);
+        part[i] = fast_exp2(mp - base_m - KA_SHIFT);
+        scale_v[i] = sees ? vs * part[i] : 0.f;
       }
 #pragma unroll
       for (int y = 0; y < 4; ++y)
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(32) kv8_attn_kernel(const __grid_constant__ Kv
         mma_f16(sum, ones, pf[y][0], pf[y][1]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) l[i] = fmaf(l[i], keep[i], sum[i]);
+      for (int i = 0; i < 2; ++i) l[i] = fmaf(l[i], keep[i], sum[i] * part[i]);
     }
     if (live && !dead && !wait_phase(full + sv, phase, &abort_flag)) failed();
     if (live) {

@@ -484,3 +484,16 @@ def test_values_apart_channel_by_channel(kind, rows):
         for gap in (0.0, 15.0, -15.0):
             check_apart(c, 64 * len(pages), rows, 128, gap)
     assert status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("rows", [1, 7])
+def test_small_weights_of_large_values(kind, dh, rows):
+    """A page that a row hardly listens to counts all the same if its values are large enough."""
+    for pages in ORDERS + [[1] + [0, 0, 1] * 30]:
+        c = Case(kind, 1, dh, [64 * len(pages)], DEV)
+        apart(c, -30, 30, pages)
+        for gap in (20.0, 30.0, 40.0, 60.0, 90.0):
+            check_apart(c, 64 * len(pages), rows, dh, gap)
+    assert status() == 0

@@ -27,13 +27,10 @@ constexpr int PICK_THREADS = 512;
 constexpr int PICK_PER = 4;            // blocks that a thread keeps the values of
 constexpr int PICK_CAP = 1024;         // continuations compared at once; at least BEAM_MAX for every warp
 
-// Blocks begin at multiples of 16 bytes, so that a row that does not is read in vectors all the same: block k of a row
-// whose first logit is `skew` logits behind such a place has logits k BLK - skew .. (k + 1) BLK - skew - 1, as far as
-// there are any.
-template <typename T>
-__device__ __forceinline__ int beam_skew(const T* row) {
-  return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16) / static_cast<int>(sizeof(T));
-}
+// Block k of a row has logits k BLK - skew .. (k + 1) BLK - skew - 1, as far as there are any.  Where all rows begin alike
+// against multiples of 16 bytes, `skew` is by how many logits they do, so that they are read in vectors all the same.
+// Where they do not, it is 0 and logits are read one by one: were the rows cut each by its own address, rows with the
+// same logits would have sums that differ by a rounding, and beams that tie would not.
 __device__ __forceinline__ float beam_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float beam_logit(const float* p) { return *p; }
 // 16 bytes of logits; `lo` and `hi` cut off what is not the row's.
@@ -60,18 +57,29 @@ __device__ __forceinline__ void beam_vector(const T* row, int t, int V, float* x
 }
 
 constexpr int PASS_WARPS = 4;
-template <typename T>
+template <typename T, bool VECTORS>
 __global__ void __launch_bounds__(32 * PASS_WARPS) beam_pass_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk,
-                                                                    const float* __restrict__ scores,
+                                                                    int skew, const float* __restrict__ scores,
                                                                     const uint8_t* __restrict__ done, float2* __restrict__ part) {
   constexpr int N = 16 / sizeof(T), PER = BLK / 32;              // logits of a vector, of a lane
   const int row = blockIdx.y, blk = blockIdx.x * PASS_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (blk >= nblk || done[row] || scores[row] == -INFINITY) return;
   const T* x = logits + row * ld;
-  const int t0 = blk * BLK - beam_skew(x) + lane * N;
+  const int t0 = blk * BLK - skew;
   float v[PER];
+  if constexpr (VECTORS) {
 #pragma unroll
-  for (int i = 0; i < PER / N; ++i) beam_vector(x, t0 + i * 32 * N, V, v + i * N);
+    for (int i = 0; i < PER / N; ++i) beam_vector(x, t0 + (i * 32 + lane) * N, V, v + i * N);
+  } else {
+    x += t0 + lane;
+    if (t0 + BLK <= V) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = beam_logit(x + i * 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = t0 + i * 32 + lane < V ? beam_logit(x + i * 32) : -INFINITY;
+    }
+  }
   float m = v[0], s = 0.f;
 #pragma unroll
   for (int i = 1; i < PER; ++i) m = fmaxf(m, v[i]);
@@ -113,7 +121,7 @@ __device__ __forceinline__ Best block_best(Best b, Best* red) {
 
 template <typename T>
 __global__ void __launch_bounds__(PICK_THREADS)
-beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int K, const float* __restrict__ scores,
+beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int skew, int K, const float* __restrict__ scores,
                  const uint8_t* __restrict__ done, int eos, const float2* __restrict__ part,
                  float* __restrict__ out_score, int64_t* __restrict__ out_parent, int64_t* __restrict__ out_token,
                  uint8_t* __restrict__ out_done) {
@@ -238,7 +246,7 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
         continue;
       }
       const T* x = logits + (row0 + j) * ld;
-      const int t0 = k * BLK - beam_skew(x) + lane;
+      const int t0 = k * BLK - skew + lane;
       x += t0;
       float v[BLK / 32];
 #pragma unroll
@@ -451,8 +459,11 @@ extern "C" int cb_beam_select(const void* logits, int64_t ld, int f32, int B, in
   auto* OD = static_cast<uint8_t*>(out_done);
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    beam_pass_kernel<T><<<grid, 32 * PASS_WARPS, 0, st>>>(x, ld, V, nblk, scores, D, P);
-    beam_pick_kernel<T><<<B, PICK_THREADS, 0, st>>>(x, ld, V, nblk, K, scores, D, eos, P, out_score, out_parent, out_token, OD);
+    const bool alike = ld * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+    const int skew = alike ? static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)) : 0;
+    if (alike) beam_pass_kernel<T, true><<<grid, 32 * PASS_WARPS, 0, st>>>(x, ld, V, nblk, skew, scores, D, P);
+    else beam_pass_kernel<T, false><<<grid, 32 * PASS_WARPS, 0, st>>>(x, ld, V, nblk, skew, scores, D, P);
+    beam_pick_kernel<T><<<B, PICK_THREADS, 0, st>>>(x, ld, V, nblk, skew, K, scores, D, eos, P, out_score, out_parent, out_token, OD);
   };
   if (f32) go(static_cast<const float*>(logits));
   else go(static_cast<const __nv_bfloat16*>(logits));

@@ -162,3 +162,16 @@ def test_pool_that_names_a_page_twice():
 def test_reorder_shared_tails(length, rows, parent):
     check_shared_tails(DEV, length, rows, parent)
     assert status() == 0
+
+
+@pytest.mark.parametrize("V", [37, 5003, 20001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_equal_rows(V, dtype):
+    """Beams with the same logits and scores tie in every continuation, wherever their rows begin in memory."""
+    logits, _, done = state(3, 8, V, dtype, DEV)
+    logits[:] = logits[::8].repeat_interleave(8, 0)
+    for wide in (V, V + 1, V + 3, V + 64):
+        rows = torch.zeros(24, wide, dtype=dtype, device=DEV)
+        for skip in sorted({0, min(3, wide - V)}):
+            rows[:, skip:skip + V] = logits
+            check_select(rows[:, skip:skip + V], torch.zeros(3, 8, device=DEV), done, 1)

@@ -26,11 +26,11 @@ struct Kv8Piece {
 };
 __device__ __forceinline__ bool kv8_piece(const Kv8Cache& c, const Kv8Rows& r, int e, int piece, int* status,
                                           Kv8Piece& out) {
-  const int first = r.row0 != nullptr ? r.row0[e] : e;
-  int n = r.row0 != nullptr ? r.row0[e + 1] - first : 1;
+  int first = e, n = 1;
   const int pos0 = r.pos0[e];
-  if (n <= 0) return false;
-  if (n > r.most || first < 0 || n > r.rows - first || pos0 < 0 || pos0 > 0x7fffffff - n - KV8_PAGE) {
+  const bool ok = r.row0 == nullptr || kv8_rows_of(r.row0, e, r.rows, r.most, first, n);
+  if (ok && n == 0) return false;
+  if (!ok || pos0 < 0 || pos0 > 0x7fffffff - n - KV8_PAGE) {
     record_status(status, ST_BOUNDS, e);
     return false;
   }

@@ -52,4 +52,15 @@ __device__ __forceinline__ int kv8_page(const Kv8Cache& c, int entry, int lp, in
   return page;
 }
 
+// The rows of entry e: row0[e] .. row0[e + 1] - 1.  False where they are more than `most`, run backwards or leave the
+// tensors' `rows`; nothing is subtracted before that is known.
+__device__ __forceinline__ bool kv8_rows_of(const int* row0, int e, int rows, int most, int& first, int& n) {
+  first = row0[e];
+  const int end = row0[e + 1];
+  n = 0;
+  if (first < 0 || end < first || end > rows || end - first > most) return false;
+  n = end - first;
+  return true;
+}
+
 }  // namespace cb

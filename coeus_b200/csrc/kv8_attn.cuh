@@ -79,11 +79,10 @@ struct Kv8Entry {
 };
 __device__ __forceinline__ Kv8Entry kv8_entry(const Kv8Attn& a, int e) {
   Kv8Entry x;
-  x.first = a.row0 != nullptr ? a.row0[e] : a.first + e;
-  x.rows = a.row0 != nullptr ? a.row0[e + 1] - x.first : 1;
+  x.first = a.first + e;
+  x.rows = 1;
   x.ctx = max(0, a.ctx[e]);
-  if (x.rows <= 0) x.rows = 0;
-  else if (x.rows > a.most || x.first < 0 || x.rows > a.rows - x.first) x.rows = -1;
+  if (a.row0 != nullptr && !kv8_rows_of(a.row0, e, a.rows, a.most, x.first, x.rows)) x.rows = -1;
   return x;
 }
 

@@ -119,9 +119,9 @@ def _spans(n: int, row0, rows: int, max_rows: int):
     at = row0.tolist()
     out = []
     for e in range(n):
+        if not 0 <= at[e] <= at[e + 1] <= min(rows, at[e] + max_rows):
+            raise ValueError(f"kv8: entry {e} has rows {at[e]} .. {at[e + 1] - 1}")
         if at[e + 1] > at[e]:
-            if at[e + 1] - at[e] > max_rows or at[e] < 0 or at[e + 1] > rows:
-                raise ValueError(f"kv8: entry {e} has rows {at[e]} .. {at[e + 1] - 1}")
             out.append((e, at[e], at[e + 1] - at[e]))
     return out
 

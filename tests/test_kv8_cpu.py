@@ -156,3 +156,16 @@ def test_first_token_inside_a_page_that_nothing_has_written(kind, size):
             assert ((y.float().cpu() - x.float()).abs() <= step + 2.0 ** -133).all()
         if row0 is not None:                               # what lies in front of the first token is zero
             assert all((t == 0).all() for t in kv8.kv8_read(*c, i32([[0, 1]], DEV), i32([64], DEV), i32([0, 9], DEV), 9, 9))
+
+
+@pytest.mark.parametrize("row0", [[0, 2, 1], [2, 1, 2], [-1, 0, 2], [0, 3, 3], [3, 3, 2], [0, 2 ** 31 - 1, 2],
+                                  [-2 ** 31, 2 ** 31 - 1, 2], [0, 2, -2 ** 31]])
+def test_row_numbers_out_of_order(row0):
+    c = Case("int8", 1, 64, [3, 3])
+    c.write([0, 0], [3, 3])
+    k = torch.zeros(2, 64)
+    for call in (lambda r: kv8.kv8_write(k, k, *c.c, c.table, i32([0, 0]), r, 2),
+                 lambda r: kv8.kv8_read(*c.c, c.table, i32([0, 0]), r, 2, 2),
+                 lambda r: kv8.kv8_attention(k, *c.c, c.table, i32([3, 3]), 1, r, 2)):
+        with pytest.raises(ValueError):
+            call(i32(row0))

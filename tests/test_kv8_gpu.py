@@ -497,3 +497,33 @@ def test_small_weights_of_large_values(kind, dh, rows):
         for gap in (20.0, 30.0, 40.0, 60.0, 90.0):
             check_apart(c, 64 * len(pages), rows, dh, gap)
     assert status() == 0
+
+
+@pytest.mark.parametrize("row0,good", [([0, 2, 1], 0), ([2, 1, 2], 1), ([-1, 0, 2], 1), ([0, 3, 3], None), ([3, 3, 2], None),
+                                       ([0, 2 ** 31 - 1, 2], None), ([-2 ** 31, 2 ** 31 - 1, 2], None),
+                                       ([0, 2, -2 ** 31], 0)])
+@pytest.mark.parametrize("group", [1, 40])
+def test_row_numbers_out_of_order(row0, good, group):
+    """Entries whose row numbers run backwards or leave the rows are recorded, each alone, and nothing of theirs is
+    written; the others are answered."""
+    c = Case("int8", 1, 64, [3, 3], DEV)
+    c.write([0, 0], [3, 3])
+    before = [t.clone() for t in c.c]
+    q = torch.randn(2, group * 64, generator=c.gen).bfloat16().to(DEV)
+    table, ctx, rows = c.table.to(DEV), i32([3, 3], DEV), i32(row0, DEV)
+    out = kv8.kv8_attention(q, *c.c, table, ctx, group, row0=rows, max_rows=2)
+    assert status() == 2
+    if good is None:
+        assert (out == 0).all()
+    else:
+        a, b = row0[good], row0[good + 1]
+        want, spread = c.plain.attention(q[a:b].cpu(), c.table[good:good + 1], [3], [b - a], group, 0.125)
+        err = (out[a:b].double().cpu() - want).abs()                     # bounds as in check_attend
+        assert (err <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * spread).all()
+        assert (out[:a] == 0).all() and (out[b:] == 0).all()
+        kv8.kv8_read(*c.c, table, i32([0, 0], DEV), rows, 2, 2)
+        assert status() == 2
+    if good is None:
+        kv8.kv8_write(q[:, :64], q[:, :64], *c.c, table, i32([0, 0], DEV), rows, 2)
+        assert status() == 2
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(before, c.c))

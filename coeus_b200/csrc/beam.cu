@@ -316,6 +316,7 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t ld, int V, int nblk, int 
 
 // ------------------------------------------------------------------------------------ pages
 constexpr int BEAM_PAGE = 64;
+constexpr int PAGES_SMEM = 200 * 1024;           // of the bitmap, at most (ops/beam.py refuses larger caches)
 
 // One CTA per request.  used: one bit per page of the cache, in shared memory.
 __global__ void __launch_bounds__(256) beam_pages_kernel(const int* __restrict__ table, int width, int K,
@@ -475,9 +476,10 @@ extern "C" int cb_beam_pages(const int* table, int width, int B, int K, const in
                              void* stream) {
   if (B < 1 || K < 1 || K > BEAM_MAX || width < 1 || pool_n < 0 || num_pages < 1) return -1;
   const int bytes = (num_pages + 31) / 32 * 4;
-  if (bytes > 200 * 1024) return -2;
+  if (bytes > PAGES_SMEM) return -2;
+  // always the same limit: one that went by the call would be lowered under another thread's launch
   if (bytes > 40 * 1024 &&
-      cudaFuncSetAttribute(beam_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      cudaFuncSetAttribute(beam_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAGES_SMEM) != cudaSuccess)
     return -4;
   beam_pages_kernel<<<B, 256, bytes, static_cast<cudaStream_t>(stream)>>>(table, width, K, parent, length, pool, pool_n,
                                                                           num_pages, out, src, dst, status);

@@ -1,5 +1,6 @@
 """The kernels of the beam search's step against its definition."""
 import math
+import threading
 
 import pytest
 import torch
@@ -175,3 +176,30 @@ def test_select_equal_rows(V, dtype):
         for skip in sorted({0, min(3, wide - V)}):
             rows[:, skip:skip + V] = logits
             check_select(rows[:, skip:skip + V], torch.zeros(3, 8, device=DEV), done, 1)
+
+
+def test_large_caches_in_two_threads():
+    """Threads whose caches differ in size, both beyond what a launch may use without asking: every launch is
+    accepted, whichever thread asked last."""
+    table, pool, total = pages_case(2, 4, [70, 20], 2, DEV)
+    n, parent = torch.tensor([70, 20], dtype=torch.int32, device=DEV), torch.tensor([[0, 0, 0, 2], [1, 1, 1, 1]], device=DEV)
+    want = beam.beam_pages(table, parent, n, pool, total)
+    state, stream = _lib.status_buffer(table.device), _lib.stream_int()
+    call, refused, wrong = _lib.entry("cb_beam_pages", "piiipppiippppp"), [], []
+
+    def work(pages):
+        got = [torch.empty_like(t) for t in want]
+        for _ in range(10000):             # the library's entry itself: the interpreter's lock would keep the calls apart
+            rc = call(table.data_ptr(), table.shape[1], 2, 4, parent.data_ptr(), n.data_ptr(), pool.data_ptr(),
+                      pool.shape[1], pages, *[t.data_ptr() for t in got], state.data_ptr(), stream)
+            if rc:
+                refused.append((pages, rc))
+        torch.cuda.synchronize()
+        wrong.extend(pages for a, b in zip(got, want) if not torch.equal(a, b))
+    threads = [threading.Thread(target=work, args=(p,)) for p in (350_000, 200 * 1024 * 8) * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not refused and not wrong, (len(refused), refused[:3], wrong)
+    assert status() == 0

@@ -33,6 +33,7 @@ def make_engine(model, **kw) -> "InferenceEngine":
 
 class InferenceEngine:
     ragged = False       # whether step() runs unequal entries as one batch
+    paged_rows = 2048    # rows of one pass over a cache in 8 bits when a prompt goes on from cached pages
 
     def __init__(self, model: DecoderLM, max_batch: int = 64, max_len: Optional[int] = None,
                  decode_splits: int = 0, use_graph: Optional[bool] = None,
@@ -256,13 +257,18 @@ class InferenceEngine:
         return self._logits(x[-1:].contiguous())[0]
 
     def prefill_slot_paged(self, slot: int, ids: torch.Tensor, total_len: int,
-                           prefix_pages: List[int]) -> torch.Tensor:
+                           prefix_pages: List[int],
+                           token_chunk: Optional[int] = None) -> torch.Tensor:
         """Like :meth:`prefill_slot`, but the first ``len(prefix_pages) * 64`` prompt tokens are
         not computed: their keys and values already sit in ``prefix_pages`` (filled by an earlier
         request with the same prefix), which the slot adopts.  The rest of the prompt runs in
         page-sized chunks, each attending to the pages before it and causally to itself; the last
         chunk is padded to a full page (rows past the prompt are computed and thrown away, their
-        cache entries are overwritten by the decode steps before anything reads them)."""
+        cache entries are overwritten by the decode steps before anything reads them).
+
+        Over a cache in 8 bits the rest runs in portions of ``token_chunk`` tokens (``paged_rows`` if
+        None; whole pages of them where it is a page or more) that attend to the cache, their own keys and
+        values included, which they see as they are stored."""
         cache, m, cfg = self.cache, self.m, self.cfg
         PG = D.PAGE
         S = ids.numel()
@@ -270,9 +276,12 @@ class InferenceEngine:
         if not 0 <= P < S:
             raise ProcessingError.invalid_input("the cached prefix must be shorter than the prompt")
         cache.adopt(slot, list(prefix_pages))
-        if cache.kind is not None:       # the rest as one entry of many rows, on top of the pages
+        if cache.kind is not None:       # portions are entries of many rows, on top of what is stored
             cache.reserve(slot, total_len)
-            x = self._entries([slot], [ids[P:]], [P])
+            n = max(1, int(token_chunk or self.paged_rows))
+            n -= n % PG if n > PG else 0
+            for c0 in range(P, S, n):
+                x = self._entries([slot], [ids[c0:c0 + n]], [c0])
             cache.set_length(slot, S)
             return self._logits(x[-1:].contiguous())[0]
         padded = P + (S - P + PG - 1) // PG * PG

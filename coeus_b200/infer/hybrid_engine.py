@@ -520,6 +520,6 @@ class HybridEngine(InferenceEngine):
         return self.step([Entry(s, p, [t], [0]) for s, t, p in
                           zip(slots.tolist(), tokens.tolist(), positions.tolist())])
 
-    def prefill_slot_paged(self, slot, ids, total_len, prefix_pages):
+    def prefill_slot_paged(self, slot, ids, total_len, prefix_pages, token_chunk=None):
         raise ProcessingError.unsupported("a prompt on cached prefix pages",
                                           "the layers' state at that point is not in the pages")

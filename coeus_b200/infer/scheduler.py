@@ -338,7 +338,8 @@ class ContinuousBatcher:
         for attempt in range(2):
             pages = self.prefix.match(r.prompt, PAGE)
             try:
-                logits = eng.prefill_slot_paged(r.slot, ids, total, pages)
+                logits = eng.prefill_slot_paged(r.slot, ids, total, pages,
+                                                token_chunk=self.token_chunk)
                 break
             except ResourceError:
                 # the pool is full of cached prefixes nobody uses right now: drop some, retry

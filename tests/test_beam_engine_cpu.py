@@ -203,3 +203,46 @@ def test_fewer_tokens_than_beams(V, K, S):
             for i, (score, tokens) in enumerate(want):
                 assert abs(float(scores[0, i]) - score) < 1e-4
                 assert out[0, i, S:].tolist() == tokens
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("pages", [0, 2])
+def test_portions_behind_cached_pages(kv, pages):
+    """The rest of a prompt goes through the layers in bounded portions, to the same cache and logits."""
+    m = model("gqa")
+    S = 250
+    ids = torch.randint(0, 61, (S,), generator=torch.Generator().manual_seed(7))
+    eng = InferenceEngine(m, max_batch=4, kv_dtype=kv)
+    eng.open_slots(4, 320)
+    eng.prefill_slot(0, ids, 260)
+    cached = eng.cache.owned[0][:pages]
+    rows = []
+    through = eng._layers
+    eng._layers = lambda x, *a, **kw: (rows.append(x.shape[0]), through(x, *a, **kw))[1]
+    want = eng.prefill_slot_paged(1, ids, 260, cached)
+    assert rows == [S - 64 * pages]
+    kept = [[t[eng.cache.owned[1]].clone() for t in eng.cache.layer(l)] for l in range(2)]
+    for chunk, most in ((64, 64), (100, 64), (128, 128), (30, 30)):
+        rows.clear()
+        got = eng.prefill_slot_paged(2, ids, 260, cached, token_chunk=chunk)
+        assert max(rows) == min(most, S - 64 * pages) and sum(rows) == S - 64 * pages
+        assert eng.cache.length(2) == S
+        if chunk >= 64:                    # pages are written whole: the same codes, sums of fp32 in another order
+            for l in range(2):
+                for a, b in zip(kept[l], eng.cache.layer(l)):
+                    b = b[eng.cache.owned[2]]
+                    if a.dtype == torch.float32:
+                        assert torch.equal(a, b)
+                    else:
+                        assert (a.view(torch.int8) != b.view(torch.int8)).float().mean() < 0.01
+            assert float((got - want).abs().max()) < 0.02 * float(want.abs().max())
+        else:                              # a page's scale may grow while it fills
+            assert float((got - want).abs().max()) < 0.08 * float(want.abs().max())
+        eng.cache.release(2)
+    b = ContinuousBatcher(InferenceEngine(m, max_batch=4, kv_dtype=kv), max_seqs=2, max_len=300,
+                          token_chunk=64, prefix_cache=True)
+    through2 = b.engine._layers
+    rows.clear()
+    b.engine._layers = lambda x, *a, **kw: (rows.append(x.shape[0]), through2(x, *a, **kw))[1]
+    rid = b.submit(ids.tolist(), 3)
+    assert len(b.run()[rid]) == 3 and max(rows) == 64

@@ -348,8 +348,11 @@ class InferenceEngine:
     def step(self, entries) -> Optional[torch.Tensor]:
         """The next tokens of several sequences (:class:`coeus_b200.ops.ragged.Entry`), cut anywhere;
         the logits ``[wanted, V]`` of the wanted places in order.  Over a cache in 8 bits they run as one
-        batch; the attention over the bf16 cache wants one
-        token per sequence, so an entry's tokens take one decode batch each."""
+        batch, in which a sequence has one entry (two would write its last page, and the page's scale, at
+        the same time); the attention over the bf16 cache wants one token per sequence, so an entry's tokens
+        take one decode batch each."""
+        if self.cache.kind is not None and len({e.slot for e in entries}) != len(entries):
+            raise ProcessingError.invalid_input("a sequence has one entry of a step over a cache in 8 bits")
         for e in entries:
             self.cache.reserve(e.slot, e.pos0 + len(e.tokens))
         if self.cache.kind is not None:

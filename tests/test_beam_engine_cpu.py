@@ -246,3 +246,17 @@ def test_portions_behind_cached_pages(kv, pages):
     b.engine._layers = lambda x, *a, **kw: (rows.append(x.shape[0]), through2(x, *a, **kw))[1]
     rid = b.submit(ids.tolist(), 3)
     assert len(b.run()[rid]) == 3 and max(rows) == 64
+
+
+def test_a_sequence_twice_in_a_step():
+    m = model()
+    eng = InferenceEngine(m, max_batch=4, kv_dtype="int8")
+    eng.open_slots(4, 128)
+    ids = torch.arange(20)
+    for slot in (0, 1):
+        eng.prefill_slot(slot, ids, 40)
+    before = [t.clone() for l in range(2) for t in eng.cache.layer(l)]
+    with pytest.raises(ProcessingError):
+        eng.step([Entry(0, 20, [5], [0]), Entry(1, 20, [6], [0]), Entry(0, 21, [7], [0])])
+    assert all(torch.equal(a, b) for a, b in zip(before, (t for l in range(2) for t in eng.cache.layer(l))))
+    assert eng.step([Entry(0, 20, [5, 7], [1]), Entry(1, 20, [6], [0])]).shape[0] == 2

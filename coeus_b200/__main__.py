@@ -283,6 +283,9 @@ def cmd_generate(store, rest: List[str]) -> dict:
                          "file (<weights>.tokenizer.json or --tokenizer=...)")
     n = int(_get(store, "max_tokens") or 16)
     beams = int(_get(store, "beams") or 1)
+    penalty = _get(store, "length_penalty")
+    if penalty is not None and beams < 2:
+        raise SystemExit("--length_penalty ranks the results of --beams=2 or more")
     engine = make_engine(model, max_batch=beams, **_kv_dtype(store))
     prompt = torch.tensor(ids, device=device)[None]
     eos = _get(store, "eos_id")
@@ -290,7 +293,6 @@ def cmd_generate(store, rest: List[str]) -> dict:
     if beams > 1:
         if temperature:
             raise SystemExit("--beams searches and --temperature samples: one of them")
-        penalty = _get(store, "length_penalty")
         found, scores = engine.beam_search(prompt, beams, n,
                                            eos_id=None if eos is None else int(eos),
                                            length_penalty=1.0 if penalty is None else float(penalty))

@@ -260,3 +260,20 @@ def test_a_sequence_twice_in_a_step():
         eng.step([Entry(0, 20, [5], [0]), Entry(1, 20, [6], [0]), Entry(0, 21, [7], [0])])
     assert all(torch.equal(a, b) for a, b in zip(before, (t for l in range(2) for t in eng.cache.layer(l))))
     assert eng.step([Entry(0, 20, [5, 7], [1]), Entry(1, 20, [6], [0])]).shape[0] == 2
+
+
+def test_length_penalty_goes_with_beams(tmp_path, capsys):
+    from coeus_b200.__main__ import main
+    from coeus_b200.checkpoint.formats import save_model
+    path = tmp_path / "m.safetensors"
+    save_model(model("gpt"), str(path))
+    args = ["generate", f"--weights={path}", "--prompt_ids=5,6,7", "--max_tokens=4", "--device=cpu"]
+    for more in (["--length_penalty=0.7"], ["--length_penalty=0.7", "--beams=1"]):
+        with pytest.raises(SystemExit):
+            main(args + more)
+    capsys.readouterr()
+    scores = []
+    for penalty in ("1.0", "0.0"):
+        main(args + ["--beams=2", f"--length_penalty={penalty}"])
+        scores.append(json.loads(capsys.readouterr().out.strip().splitlines()[-1])["score"])
+    assert abs(scores[0] * 4 - scores[1]) < 1e-5 * abs(scores[1])       # four tokens each: divided by 4, or by 1

@@ -13,9 +13,14 @@ bits of every number however small.
 
 The entries of a call are sequences: entry ``e`` has page-table row ``e``.  With ``row0 [n + 1]`` it
 owns rows ``row0[e] .. row0[e + 1] - 1`` of the row-wise tensors, at most ``max_rows`` of them
-(possibly none); without, row ``e`` alone.  An entry whose rows, positions or pages are out of range is
-skipped and recorded in the status word (:func:`coeus_b200.ops._lib.check_status`).  Entries of one
-:func:`kv8_write` must not write the same page.
+(possibly none); without, row ``e`` alone.  Entries of one :func:`kv8_write` must not write the same page.
+
+What is out of range is refused on the CPU.  The kernels record it in the status word
+(:func:`coeus_b200.ops._lib.check_status`) and touch nothing outside the tensors: an entry whose row
+numbers run backwards, leave the rows or are more than ``max_rows``, or whose first position is negative or
+next to 2^31, is skipped; a page that the table or the cache does not have is left out, so that its
+tokens are neither written nor read and its keys take no part in the softmax (a row that sees tokens, but none
+that is there, gets NaN); a context that goes beyond the table ends with it.
 """
 from __future__ import annotations
 
@@ -272,7 +277,14 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     """``q [rows, nh * dh]`` -> ``[rows, nh * dh]``.  Entry ``e`` holds ``ctx_len[e]`` tokens, its rows
     are the last of them and every row sees the tokens up to itself; a row that sees none gets zeros, and
     so do rows that no entry owns.  Query head ``h`` reads cache head ``h // (nh // heads)``; ``scale``
-    defaults to ``1 / sqrt(dh)``."""
+    defaults to ``1 / sqrt(dh)``.
+
+    The kernels hold queries (against the largest number of their row) and weights in fp16 and every sum in
+    fp32.  A weight is off by 2^-11 of itself; one below 2^-23 of its row's largest may lose digits, one
+    below 2^-34 may count as nothing in a channel where the values beside it are no larger, and so may a value
+    that is 2^60 below another one of its row and head.  Which of the two kernels runs, for few rows or for many,
+    goes by the rows that share a cache head and by the entries, heads and width of the page table, not by
+    the contexts: they agree up to these roundings."""
     pages, heads, dh, n, device = _check("kv8_attention", k_cache, v_cache, k_scale, v_scale,
                                          page_table, ctx_len, row0, max_rows)
     if nh < 1 or nh % heads:

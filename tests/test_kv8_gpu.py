@@ -527,3 +527,32 @@ def test_row_numbers_out_of_order(row0, good, group):
         kv8.kv8_write(q[:, :64], q[:, :64], *c.c, table, i32([0, 0], DEV), rows, 2)
         assert status() == 2
         assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(before, c.c))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [1, 3, 100])
+def test_pages_that_are_not_there(kind, rows):
+    """A page that the cache does not have takes no part, a row that sees no other gets NaN, and a context beyond
+    the table ends with it; all of it is recorded."""
+    n = 400
+    c = Case(kind, 1, 64, [n], DEV, width=7)
+    c.write([0], [n])
+    q = torch.randn(rows, 64, generator=c.gen).bfloat16()
+    table, first, most = c.table.to(DEV), None if rows == 1 else i32([0, rows], DEV), rows
+    call = lambda t, ctx: kv8.kv8_attention(q.to(DEV), *c.c, t, i32([ctx], DEV), 1, first, most).double().cpu()
+    k, v = (x.view(n, 64) for x in c.plain.read(c.table, [0], [n]))
+    gone = table.clone()
+    gone[0, 0], gone[0, 2], gone[0, 5] = -1, 10 ** 6, 2 ** 31 - 1
+    got = call(gone, n)
+    assert status() == 2
+    here = torch.tensor([p // 64 not in (0, 2, 5) for p in range(n)])
+    for i in range(rows):
+        mine = here & (torch.arange(n) <= n - rows + i)
+        w = torch.softmax(k[mine] @ q[i].double() * 0.125, 0)[:, None]
+        want, spread = (w * v[mine]).sum(0), (w * v[mine].abs()).sum(0)
+        assert ((got[i] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * spread).all()    # as in check_attend
+    assert torch.isnan(call(torch.full_like(gone, -1), n)).all() and status() == 2
+    short = table[:, :6].contiguous()                      # 384 tokens
+    got = call(short, 500)
+    assert status() == 2
+    assert torch.equal(got, call(short, 384)) and status() == 0

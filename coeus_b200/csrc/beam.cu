@@ -4,8 +4,9 @@
 // Selection.  Continuation t of beam j is worth score_j + logit_jt - logsumexp(logit_j); a beam that has
 // ended continues with the end token alone, at its own score.  Taken are the K largest, equal ones by
 // the lowest j V + t.  The values are formed in fp64: they differ between beams by less than fp32 resolves.
-// 32 requests of 8 beams of 100003 fp32 logits: 16.5 us for the pass (0.71 of the copy rate), 20 for the choice, which is a
-// chain of reductions of one CTA per request and does not get shorter with fewer bytes.
+// 32 requests of 8 beams, 6 of them going on, of 100008 fp32 logits (77 MB): 17.4 us for the pass (0.67 of the copy rate;
+// 18.1 for rows of 100003, read one by one), 23 for the choice, which is a chain of reductions of one CTA per request and
+// does not get shorter with fewer bytes; 8 of 8 beams in bf16 (51 MB): 21 and 25, bound by the exponentials.
 //   pass   one read of the logits: maximum and sum of exponentials of every block of BLK of a row.
 //   pick   one CTA per request.  The K best continuations lie in the K blocks whose best ones are
 //          the best (equal ones by the lowest place): each of those holds one that precedes whatever lies in

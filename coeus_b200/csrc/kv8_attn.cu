@@ -11,7 +11,7 @@
 // many CTAs as shared memory holds share an SM (dh 128: six) and know nothing of each other.  Warps of one CTA that
 // took the pages of a tile in turn and merged their parts waited for one another (64 sequences of 1000 to 8200, 32
 // heads over 8 of 128: 175 to 255 us, so 124).  64 sequences of 4096 with these heads: 101 us and 12 for the merge, 0.81 of
-// the copy rate; 64 of 2048 with 16 heads of 64: 57 and 16, 0.72; one of 131072: 49 and 16, 0.83.  What it waits for is
+// the copy rate; 64 of 2048 with 16 heads of 64: 57 and 16, 0.72; one of 131072: 50 and 17, 0.82.  What it waits for is
 // latency (36 % of the issue slots are used): the steps of a page follow one another and there are no more warps.
 //
 // Both products are transposed, S^T = K Q^T and O^T = V^T P^T (mma m16n8k16 in fp16, fp32 sums), so that

@@ -17,8 +17,8 @@
 // scale is far below that of the sums (KB_NEAR) but its scores are not, m is lowered to md + ev: its values may be all that
 // some channels have.  A page of a tile is 2 x 64 x 128 dh
 // multiply-adds and 8192 exponentials; what bounds it is the chain of score product, softmax and value product, two tiles
-// an SM in turn.  Four sequences of 8192 with 512 rows each, 32 heads over 8 of 128: 448 us and 18 for the merge, 0.35 of
-// the bf16 rate.  Four of 2000 to 8200 with 301 to 700 rows: 351 us in all, 469 with one CTA an SM and one issuing thread;
+// an SM in turn.  Four sequences of 8192 with 512 rows each, 32 heads over 8 of 128: 443 us and 18 for the merge, 0.35 of
+// the bf16 rate.  Four of 2000 to 8200 with 301 to 700 rows: 348 us in all (377 with the maxima raised for every page), 469 with one CTA an SM and one issuing thread;
 // 200 with nothing but the products and the barriers.  Keys and values handed over separately: 360.
 #include "kv8_attn.cuh"
 

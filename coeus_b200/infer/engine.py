@@ -41,8 +41,10 @@ class InferenceEngine:
         """``use_graph``: capture the decode step in a CUDA graph and replay it per token (default:
         on for CUDA models whose positions are not taken from a host-indexed table).  Positions
         then live in device buffers that are never reallocated.  ``kv_dtype``: ``"int8"`` or
-        ``"e4m3"`` keeps the cache in 8 bits (heads of 64 or 128), half the bytes that a token reads;
-        a prompt's own attention still sees its keys and values as computed."""
+        ``"e4m3"`` keeps the cache in 8 bits (heads of 64 or 128), half the bytes that a token reads.  A
+        prompt that runs in one pass sees its keys and values as computed; in chunks (``token_chunk``) it sees
+        those of the earlier chunks as they are stored, and behind cached pages
+        (:meth:`prefill_slot_paged`) all of them."""
         self.m = model
         self.cfg = model.cfg
         if kv_dtype is not None and (kv_dtype not in kv8.KINDS or

@@ -10,15 +10,15 @@
 //                 reads them; the running maximum, the sum, and at the end the tile's rows
 //
 // The scale 2^ev of a page's values goes into the weights: with z = s + ev (s the score in units of log2) and m a
-// running maximum of z, the weights are P = 2^(z - m).  The denominator has a maximum of its own, md of s alone, and sums
-// 2^(m - ev - md) P = 2^(s - md): o = 2^(m - md) sum P code / sum 2^(s - md).  So pages of any scales add up in one
+// running maximum of z, the weights are P = 2^(z - m).  The denominator has a maximum of its own, md of s alone, and
+// sums 2^(m - ev - md) P = 2^(s - md): o = 2^(m - md) sum P code / sum 2^(s - md).  So pages of any scales add up in one
 // accumulator, and a page without values, whose ev says nothing, counts for the denominator alone.  m and md are whole
-// numbers, only raised when they are exceeded by more than KB_LAG, and the sums so far are multiplied then.  Where a page's
-// scale is far below that of the sums (KB_NEAR) but its scores are not, m is lowered to md + ev: its values may be all that
-// some channels have.  A page of a tile is 2 x 64 x 128 dh
-// multiply-adds and 8192 exponentials; what bounds it is the chain of score product, softmax and value product, two tiles
-// an SM in turn.  Four sequences of 8192 with 512 rows each, 32 heads over 8 of 128: 443 us and 18 for the merge, 0.35 of
-// the bf16 rate.  Four of 2000 to 8200 with 301 to 700 rows: 348 us in all (377 with the maxima raised for every page), 469 with one CTA an SM and one issuing thread;
+// numbers, only raised when they are exceeded by more than KB_LAG, and the sums so far are multiplied then.  Where a
+// page's scale is far below that of the sums (KB_NEAR) but its scores are not, m is lowered to md + ev: its values may
+// be all that some channels have.  A page of a tile is 2 x 64 x 128 dh multiply-adds and 8192 exponentials; what bounds
+// it is the chain of score product, softmax and value product, two tiles an SM in turn.  Four sequences of 8192 with 512
+// rows each, 32 heads over 8 of 128: 443 us and 18 for the merge, 0.35 of the bf16 rate.  Four of 2000 to 8200 with 301
+// to 700 rows: 348 us in all (377 with the maxima raised for every page), 469 with one CTA an SM and one issuing thread;
 // 200 with nothing but the products and the barriers.  Keys and values handed over separately: 360.
 #include "kv8_attn.cuh"
 
